@@ -30,6 +30,31 @@ _vp = ctypes.c_void_p
 _i = ctypes.c_int
 _sz = ctypes.c_size_t
 
+_ll = ctypes.c_longlong
+
+
+class PagedCache(ctypes.Structure):
+    """ca_paged_cache of the public header."""
+    _fields_ = ([(n, _vp) for n in ("k", "v", "table", "lengths", "starts")]
+                + [(n, _ll) for n in ("page_stride", "head_stride", "row_stride", "table_stride")]
+                + [(n, _i) for n in ("dtype", "heads", "head_dim", "page_size", "num_pages",
+                                     "pages_per_seq", "batch", "tokens")])
+
+
+class Rotary(ctypes.Structure):
+    """ca_rotary of the public header."""
+    _fields_ = ([(n, _vp) for n in ("q", "k", "q_out", "k_out", "positions", "turns")]
+                + [(n, _ll) for n in ("q_token_stride", "q_head_stride", "k_token_stride",
+                                      "k_head_stride", "q_out_token_stride", "q_out_head_stride",
+                                      "k_out_token_stride", "k_out_head_stride")]
+                + [("magnitude", ctypes.c_float)]
+                + [(n, _i) for n in ("positions64", "half", "inverse", "dtype", "tokens", "q_heads",
+                                     "k_heads", "head_dim", "rotary_dim")])
+
+
+_cache_p = ctypes.POINTER(PagedCache)
+_rotary_p = ctypes.POINTER(Rotary)
+
 # name -> (restype, argtypes); one entry per declaration in the public header
 SIGNATURES = {
     "ca_abi_version": (_i, []),
@@ -68,6 +93,13 @@ SIGNATURES = {
     "ca_bf16_shadow": (_i, [_vp, _i, _vp, _i, _vp]),
     "ca_swiglu_fwd_f32": (_i, [_vp, _vp, _i, _i, _vp]),
     "ca_swiglu_bwd_f32": (_i, [_vp, _vp, _vp, _i, _i, _vp]),
+    "ca_paged_attention_workspace_bytes": (_sz, [_i] * 8),
+    "ca_paged_attention": (_i, [_cache_p, _vp, _ll, _ll, _i, _vp, _vp, _ll, _ll, _vp, _ll, _ll, _i,
+                                _i, _i, _vp, _sz, _vp]),
+    "ca_evict": (_i, [_cache_p, _vp, _ll, _ll, _i, _i, _i, _i, _vp, _ll, _vp, _vp, _vp, _vp]),
+    "ca_rotary_embedding": (_i, [_rotary_p, _vp]),
+    "ca_rotary_append": (_i, [_rotary_p, _vp, _ll, _ll, _cache_p, _vp]),
+    "ca_int4_linear": (_i, [_vp, _ll, _vp, _vp, _vp, _vp, _ll, _i, _i, _i, _i, _i, _vp]),
     "ca_timing_enable": (_i, [_i]),
     "ca_timing_read": (_i, [ctypes.POINTER(ctypes.c_double), ctypes.POINTER(_i), _i]),
     "ca_debug_set_splits": (_i, [_i, _i, _i]),

@@ -16,7 +16,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libca_hip.so")
 SOURCES = ["ca_fwd.hip", "ca_bwd.hip", "ca_bwd_dkdv.hip", "ca_weights.hip", "ca_norm.hip",
-           "ca_optim.hip", "ca_swiglu.hip", "ca_abi.hip", "ca_noalloc.hip"]
+           "ca_optim.hip", "ca_swiglu.hip", "ca_paged.hip", "ca_evict.hip", "ca_rotary.hip",
+           "ca_int4.hip", "ca_abi.hip", "ca_serving_abi.hip", "ca_noalloc.hip"]
 ARCH = os.environ.get("CA_OFFLOAD_ARCH", "gfx950")
 TORCH_SOURCE = "ca_torch.cpp"
 TORCH_EXT = os.path.join(HERE, "_ca_torch.so")

@@ -1,0 +1,345 @@
+// C ABI of the generation operators: attention over a paged cache, eviction from
+// it, rotary positions, 4-bit products.  Declarations:
+// include/continuum_attention_amd.h.
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "ca_evict.h"
+#include "ca_int4.h"
+#include "ca_paged.h"
+#include "ca_rotary.h"
+
+namespace {
+
+using ca::set_error;
+
+bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+int element_bytes(int dtype) {
+  return dtype == CA_DTYPE_F32 ? 4 : dtype == CA_DTYPE_BF16 || dtype == CA_DTYPE_F16 ? 2 : 0;
+}
+constexpr int kMaxSlots = 1 << 30;  // slots a sequence may have: tile ends stay below 2^31
+
+// A cache's numbers and pointers; `op` names the caller.
+int check_cache(const char* op, const ca_paged_cache* c, bool starts = true) {
+  if (!c) return set_error(CA_ERR_INVALID, "%s: null cache", op);
+  const int e = element_bytes(c->dtype);
+  if (!e) return set_error(CA_ERR_INVALID, "%s: unknown dtype %d", op, c->dtype);
+  if (c->batch <= 0 || c->heads <= 0 || c->tokens < 0 || c->num_pages <= 0 || c->page_size <= 0 ||
+      c->pages_per_seq <= 0 || c->head_dim <= 0)
+    return set_error(CA_ERR_INVALID,
+                     "%s: invalid sizes batch=%d heads=%d tokens=%d num_pages=%d page_size=%d pages_per_seq=%d "
+                     "head_dim=%d", op, c->batch, c->heads, c->tokens, c->num_pages, c->page_size,
+                     c->pages_per_seq, c->head_dim);
+  if (c->head_dim % 8 || c->head_dim > 128)
+    return set_error(CA_ERR_UNSUPPORTED, "%s: head dim %d (multiples of 8 up to 128)", op, c->head_dim);
+  if ((long long)c->pages_per_seq * c->page_size > kMaxSlots)
+    return set_error(CA_ERR_UNSUPPORTED, "%s: %d pages of %d slots per sequence exceed 2^30", op,
+                     c->pages_per_seq, c->page_size);
+  if (c->table_stride < c->pages_per_seq)
+    return set_error(CA_ERR_INVALID, "%s: table stride %lld below %d pages per sequence", op,
+                     c->table_stride, c->pages_per_seq);
+  if (!c->k || !c->v || !c->table || !c->lengths || (starts && !c->starts))
+    return set_error(CA_ERR_INVALID, "%s: null pointer", op);
+  if (!aligned(c->table, 4) || !aligned(c->lengths, 4) || !aligned(c->starts, 4))
+    return set_error(CA_ERR_INVALID, "%s: table, lengths and starts must be 4-byte aligned", op);
+  if (!aligned(c->k, 16) || !aligned(c->v, 16) || c->page_stride * e % 16 || c->head_stride * e % 16 ||
+      c->row_stride * e % 16)
+    return set_error(CA_ERR_INVALID, "%s: cache rows must be 16-byte aligned", op);
+  return CA_OK;
+}
+
+ca::PagedCache kernel_cache(const ca_paged_cache& c) {
+  ca::PagedCache k;
+  k.k = c.k;
+  k.v = c.v;
+  k.page_stride = c.page_stride;
+  k.head_stride = c.head_stride;
+  k.row_stride = c.row_stride;
+  k.table = c.table;
+  k.lengths = c.lengths;
+  k.starts = c.starts;
+  k.table_stride = c.table_stride;
+  k.pages_per_seq = c.pages_per_seq;
+  k.num_pages = c.num_pages;
+  k.heads = c.heads;
+  k.D = c.head_dim;
+  k.batch = c.batch;
+  k.div = ca::page_div(c.page_size);
+  return k;
+}
+
+// How the attention's grid is cut.  max_new and max_length only size it: the
+// kernels read what is there from the device and walk all of it.
+struct AttnPlan {
+  int wave_rows, row_tiles, splits, split_keys;
+};
+constexpr int kOwnedKeys = 30;    // keys of a tile (ca_paged.hip)
+constexpr int kTargetGroups = 1024;  // four work groups on each of 256 CUs
+constexpr int kLeastTiles = 8;    // tiles of a split
+constexpr int kMostSplits = 128;
+
+size_t partial_bytes(int splits, int tokens, int heads, int D) {
+  return splits > 1 ? (size_t)splits * tokens * heads * (D + 2) * sizeof(float) : 0;
+}
+AttnPlan attn_plan(int batch, int kv_heads, int heads, int D, int tokens, int max_new, int max_length) {
+  const long long rows = (long long)std::max(1, std::min(max_new, tokens)) * (heads / kv_heads);
+  AttnPlan p;
+  p.wave_rows = rows <= 16 ? 1 : 4;
+  const long long tiles = (rows + 16 * p.wave_rows - 1) / (16 * p.wave_rows);
+  const long long slices = (long long)batch * kv_heads;
+  const int key_tiles = std::max(1, (max_length + kOwnedKeys - 1) / kOwnedKeys);
+  long long splits = std::max<long long>(1, kTargetGroups / std::max<long long>(1, slices * tiles));
+  splits = std::min<long long>(splits, std::max(1, key_tiles / kLeastTiles));
+  splits = std::min<long long>(splits, kMostSplits);
+  const size_t cap = ca_workspace_cap();
+  while (splits > 1 && cap && partial_bytes((int)splits, tokens, heads, D) > cap) --splits;
+  const int per = (key_tiles + (int)splits - 1) / (int)splits;
+  p.splits = (key_tiles + per - 1) / per;
+  p.split_keys = per * kOwnedKeys;
+  // at most 2^31 - 1 work groups
+  p.row_tiles = (int)std::max<long long>(1, std::min<long long>(tiles, ((1ll << 31) - 1) / (slices * p.splits)));
+  return p;
+}
+size_t stats_bytes(int tokens, int heads) { return ((size_t)tokens * heads * 2 * sizeof(float) + 255) & ~(size_t)255; }
+
+}  // namespace
+
+extern "C" {
+
+size_t ca_paged_attention_workspace_bytes(int batch, int kv_heads, int heads, int head_dim, int tokens,
+                                          int max_new, int max_length, int with_sums) {
+  if (batch <= 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || head_dim <= 0 || tokens <= 0) return 0;
+  const AttnPlan p = attn_plan(batch, kv_heads, heads, head_dim, tokens, max_new, max_length);
+  return partial_bytes(p.splits, tokens, heads, head_dim) + (with_sums ? stats_bytes(tokens, heads) : 0);
+}
+
+int ca_paged_attention(const ca_paged_cache* cache, const void* q, long long q_token_stride,
+                       long long q_head_stride, int heads, const float* log_gain, void* out,
+                       long long out_token_stride, long long out_head_stride, float* sums,
+                       long long sums_batch_stride, long long sums_head_stride, int sums_len, int max_new,
+                       int max_length, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* op = "ca_paged_attention";
+  int rc = check_cache(op, cache);
+  if (rc) return rc;
+  if (heads <= 0 || heads % cache->heads)
+    return set_error(CA_ERR_INVALID, "%s: %d query heads over %d key heads", op, heads, cache->heads);
+  if (cache->tokens == 0) return CA_OK;
+  if (!q || !log_gain || !out) return set_error(CA_ERR_INVALID, "%s: null pointer", op);
+  const int e = element_bytes(cache->dtype);
+  if (!aligned(q, 16) || q_token_stride * e % 16 || q_head_stride * e % 16)
+    return set_error(CA_ERR_INVALID, "%s: query rows must be 16-byte aligned", op);
+  if (!aligned(out, 16) || out_token_stride * e % 16 || out_head_stride * e % 16)
+    return set_error(CA_ERR_INVALID, "%s: output rows must be 16-byte aligned", op);
+  if (!aligned(log_gain, 4) || !aligned(sums, 4))
+    return set_error(CA_ERR_INVALID, "%s: log_gain and sums must be 4-byte aligned", op);
+  if ((long long)cache->tokens * heads * cache->head_dim > (1ll << 31) - 1)
+    return set_error(CA_ERR_UNSUPPORTED, "%s: %d tokens of %d heads exceed 2^31 elements", op, cache->tokens, heads);
+  if ((long long)cache->batch * cache->heads > (1 << 24))
+    return set_error(CA_ERR_UNSUPPORTED, "%s: %d sequences of %d heads exceed 2^24", op, cache->batch, cache->heads);
+  if (max_new < 0 || max_length < 0 || sums_len < 0)
+    return set_error(CA_ERR_INVALID, "%s: negative max_new, max_length or sums_len", op);
+  max_length = std::min(max_length, cache->pages_per_seq * cache->page_size);
+  const size_t need = ca_paged_attention_workspace_bytes(cache->batch, cache->heads, heads, cache->head_dim,
+                                                         cache->tokens, max_new, max_length, sums != nullptr);
+  if (need && (!workspace || workspace_bytes < need))
+    return set_error(CA_ERR_WORKSPACE, "%s: workspace of %zu bytes required, %zu given", op, need, workspace_bytes);
+  if (!aligned(workspace, 16)) return set_error(CA_ERR_INVALID, "%s: workspace must be 16-byte aligned", op);
+
+  const AttnPlan p = attn_plan(cache->batch, cache->heads, heads, cache->head_dim, cache->tokens, max_new, max_length);
+  ca::PagedAttnIO io;
+  io.c = kernel_cache(*cache);
+  io.q = q;
+  io.out = out;
+  io.q_ts = q_token_stride;
+  io.q_hs = q_head_stride;
+  io.o_ts = out_token_stride;
+  io.o_hs = out_head_stride;
+  io.log_gain = log_gain;
+  char* ws = static_cast<char*>(workspace);
+  io.stats = nullptr;
+  if (sums) {
+    io.stats = reinterpret_cast<float*>(ws);
+    ws += stats_bytes(cache->tokens, heads);
+  }
+  const long long rows = (long long)cache->tokens * heads;
+  io.part_o = reinterpret_cast<float*>(ws);
+  io.part_ml = io.part_o + (p.splits > 1 ? p.splits * rows * cache->head_dim : 0);
+  io.sums = sums;
+  io.sums_bs = sums_batch_stride;
+  io.sums_hs = sums_head_stride;
+  io.sums_len = sums_len;
+  io.tokens = cache->tokens;
+  io.Hq = heads;
+  io.group = heads / cache->heads;
+  io.splits = p.splits;
+  io.split_keys = p.split_keys;
+  io.row_tiles = p.row_tiles;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  hipError_t err = ca::launch_paged_attention(io, cache->dtype, p.wave_rows, s);
+  if (err == hipSuccess && p.splits > 1) err = ca::launch_paged_combine(io, cache->dtype, s);
+  if (err == hipSuccess && sums) err = ca::launch_paged_sums(io, cache->dtype, max_length, s);
+  if (err != hipSuccess) return set_error(CA_ERR_HIP, "%s launch: %s", op, hipGetErrorString(err));
+  return CA_OK;
+}
+
+int ca_evict(const ca_paged_cache* cache, const float* sums, long long sums_batch_stride,
+             long long sums_head_stride, int sums_len, int budget, int sinks, int recent,
+             const int* new_table, long long new_table_stride, int* kept, float* new_sums,
+             int* new_lengths, void* stream) {
+  const char* op = "ca_evict";
+  int rc = check_cache(op, cache, false);
+  if (rc) return rc;
+  if (!sums || !new_table || !kept || !new_sums || !new_lengths) return set_error(CA_ERR_INVALID, "%s: null pointer", op);
+  if (!aligned(sums, 4) || !aligned(new_table, 4) || !aligned(kept, 4) || !aligned(new_sums, 4) || !aligned(new_lengths, 4))
+    return set_error(CA_ERR_INVALID, "%s: pointers must be 4-byte aligned", op);
+  if (budget <= 0 || sinks < 0 || recent < 0 || (long long)sinks + recent > budget)
+    return set_error(CA_ERR_INVALID, "%s: budget %d must be positive and hold %d sinks and %d recent slots", op,
+                     budget, sinks, recent);
+  if (sums_len < 0) return set_error(CA_ERR_INVALID, "%s: negative sums_len", op);
+  if (new_table_stride <= 0 || new_table_stride < (budget + (long long)cache->page_size - 1) / cache->page_size)
+    return set_error(CA_ERR_INVALID, "%s: %lld new pages of %d slots do not hold %d", op, new_table_stride,
+                     cache->page_size, budget);
+  if ((long long)cache->batch * cache->heads > (1 << 24))
+    return set_error(CA_ERR_UNSUPPORTED, "%s: %d sequences of %d heads exceed 2^24", op, cache->batch, cache->heads);
+  ca::EvictIO io;
+  io.c = kernel_cache(*cache);
+  io.sums = sums;
+  io.sums_bs = sums_batch_stride;
+  io.sums_hs = sums_head_stride;
+  io.sums_len = sums_len;
+  io.budget = budget;
+  io.sinks = sinks;
+  io.recent = recent;
+  io.new_table = new_table;
+  io.new_table_stride = new_table_stride;
+  io.kept = kept;
+  io.new_sums = new_sums;
+  io.new_lengths = new_lengths;
+  io.esize = element_bytes(cache->dtype);
+  io.row_pieces = cache->head_dim * io.esize / 16;
+  hipError_t err = ca::launch_evict(io, reinterpret_cast<hipStream_t>(stream));
+  if (err != hipSuccess) return set_error(CA_ERR_HIP, "%s launch: %s", op, hipGetErrorString(err));
+  return CA_OK;
+}
+
+static int rotary_io(const char* op, const ca_rotary* r, bool cached, ca::RotaryIO& io) {
+  if (!r) return set_error(CA_ERR_INVALID, "%s: null argument", op);
+  const int e = element_bytes(r->dtype);
+  if (!e) return set_error(CA_ERR_INVALID, "%s: unknown dtype %d", op, r->dtype);
+  if (r->tokens < 0 || r->q_heads < 0 || r->k_heads < 0 || r->q_heads + (long long)r->k_heads <= 0 || r->head_dim <= 0)
+    return set_error(CA_ERR_INVALID, "%s: invalid sizes tokens=%d heads=%d,%d head_dim=%d", op, r->tokens, r->q_heads,
+                     r->k_heads, r->head_dim);
+  if (r->rotary_dim <= 0 || r->rotary_dim % 2 || r->rotary_dim > r->head_dim || r->head_dim % 2)
+    return set_error(CA_ERR_INVALID, "%s: rotary_dim %d of head dim %d (both even)", op, r->rotary_dim, r->head_dim);
+  if ((long long)r->tokens * (r->q_heads + 2ll * r->k_heads) * r->head_dim > (1ll << 38))
+    return set_error(CA_ERR_UNSUPPORTED, "%s: %d tokens of %d heads exceed 2^38 elements", op, r->tokens,
+                     r->q_heads + r->k_heads);
+  if (r->tokens == 0) return CA_OK;
+  if ((r->q_heads && (!r->q || !r->q_out)) || (r->k_heads && (!r->k || (!cached && !r->k_out))) || !r->positions || !r->turns)
+    return set_error(CA_ERR_INVALID, "%s: null pointer", op);
+  if (!aligned(r->turns, 8) || !aligned(r->positions, r->positions64 ? 8 : 4) || !aligned(r->q, e) || !aligned(r->k, e) ||
+      !aligned(r->q_out, e) || !aligned(r->k_out, e))
+    return set_error(CA_ERR_INVALID, "%s: misaligned pointer", op);
+  io.q = r->q;
+  io.k = r->k;
+  io.v = nullptr;
+  io.q_out = r->q_out;
+  io.k_out = r->k_out;
+  io.q_ts = r->q_token_stride;
+  io.q_hs = r->q_head_stride;
+  io.k_ts = r->k_token_stride;
+  io.k_hs = r->k_head_stride;
+  io.v_ts = io.v_hs = 0;
+  io.qo_ts = r->q_out_token_stride;
+  io.qo_hs = r->q_out_head_stride;
+  io.ko_ts = r->k_out_token_stride;
+  io.ko_hs = r->k_out_head_stride;
+  io.positions = r->positions;
+  io.turns = r->turns;
+  io.magnitude = r->magnitude;
+  io.positions64 = r->positions64;
+  io.R = r->rotary_dim;
+  io.D = r->head_dim;
+  io.Hq = r->q_heads;
+  io.Hk = r->k_heads;
+  io.tokens = r->tokens;
+  io.half = r->half;
+  io.inverse = r->inverse;
+  io.head_chunks = 1;
+  auto rows16 = [&](const void* p, long long ts, long long hs) { return aligned(p, 16) && ts * e % 16 == 0 && hs * e % 16 == 0; };
+  io.aligned16 = (!io.Hq || (rows16(io.q, io.q_ts, io.q_hs) && rows16(io.q_out, io.qo_ts, io.qo_hs))) &&
+                 (!io.Hk || (rows16(io.k, io.k_ts, io.k_hs) && (cached || rows16(io.k_out, io.ko_ts, io.ko_hs))));
+  io.c = ca::PagedCache{};
+  return CA_OK;
+}
+
+int ca_rotary_embedding(const ca_rotary* r, void* stream) {
+  const char* op = "ca_rotary_embedding";
+  ca::RotaryIO io;
+  int rc = rotary_io(op, r, false, io);
+  if (rc || r->tokens == 0) return rc;
+  hipError_t err = ca::launch_rotary(io, r->dtype, reinterpret_cast<hipStream_t>(stream));
+  if (err != hipSuccess) return set_error(CA_ERR_HIP, "%s launch: %s", op, hipGetErrorString(err));
+  return CA_OK;
+}
+
+int ca_rotary_append(const ca_rotary* r, const void* v, long long v_token_stride, long long v_head_stride,
+                     const ca_paged_cache* cache, void* stream) {
+  const char* op = "ca_rotary_append";
+  ca::RotaryIO io;
+  int rc = rotary_io(op, r, true, io);
+  if (rc) return rc;
+  rc = check_cache(op, cache);
+  if (rc) return rc;
+  if (cache->dtype != r->dtype || cache->heads != r->k_heads || cache->head_dim != r->head_dim || cache->tokens != r->tokens)
+    return set_error(CA_ERR_INVALID, "%s: the cache's dtype, heads, head dim or tokens differ", op);
+  if (r->inverse) return set_error(CA_ERR_INVALID, "%s: inverse has no meaning here", op);
+  if (r->tokens == 0) return CA_OK;
+  const int e = element_bytes(r->dtype);
+  if (!v || !aligned(v, e)) return set_error(CA_ERR_INVALID, "%s: null or misaligned values", op);
+  io.v = v;
+  io.v_ts = v_token_stride;
+  io.v_hs = v_head_stride;
+  io.aligned16 = io.aligned16 && aligned(v, 16) && v_token_stride * e % 16 == 0 && v_head_stride * e % 16 == 0;
+  io.c = kernel_cache(*cache);
+  hipError_t err = ca::launch_rotary(io, r->dtype, reinterpret_cast<hipStream_t>(stream));
+  if (err != hipSuccess) return set_error(CA_ERR_HIP, "%s launch: %s", op, hipGetErrorString(err));
+  return CA_OK;
+}
+
+int ca_int4_linear(const void* x, long long x_stride, const unsigned* codes, const void* scales, const void* zeros,
+                   void* y, long long y_stride, int dtype, int M, int N, int K, int group, void* stream) {
+  const char* op = "ca_int4_linear";
+  const int e = element_bytes(dtype);
+  if (!e) return set_error(CA_ERR_INVALID, "%s: unknown dtype %d", op, dtype);
+  if (M < 0 || N <= 0 || K <= 0) return set_error(CA_ERR_INVALID, "%s: invalid shape M=%d N=%d K=%d", op, M, N, K);
+  if (group != 32 && group != 64 && (group <= 0 || group % 128))
+    return set_error(CA_ERR_UNSUPPORTED, "%s: groups of %d columns (32, 64 or a multiple of 128)", op, group);
+  if ((long long)N * ((K + 127) / 128 * 128ll) > (1ll << 38) || M > (1 << 19) || K > (1 << 30) || N > (1 << 30))
+    return set_error(CA_ERR_UNSUPPORTED, "%s: M=%d N=%d K=%d too large", op, M, N, K);
+  if (x_stride < K || y_stride < N) return set_error(CA_ERR_INVALID, "%s: row strides below the rows' lengths", op);
+  if (M == 0) return CA_OK;
+  if (!x || !codes || !scales || !y) return set_error(CA_ERR_INVALID, "%s: null pointer", op);
+  if (!aligned(codes, 16) || !aligned(x, e) || !aligned(scales, e) || !aligned(zeros, e) || !aligned(y, e))
+    return set_error(CA_ERR_INVALID, "%s: misaligned pointer", op);
+  ca::Int4IO io;
+  io.x = x;
+  io.codes = codes;
+  io.scales = scales;
+  io.zeros = zeros;
+  io.y = y;
+  io.x_rs = x_stride;
+  io.y_rs = y_stride;
+  io.M = M;
+  io.N = N;
+  io.K = K;
+  io.group = group;
+  io.row_words = (K + 127) / 128 * 16;
+  io.x_aligned = aligned(x, 16) && x_stride * e % 16 == 0;
+  hipError_t err = ca::launch_int4(io, dtype, reinterpret_cast<hipStream_t>(stream));
+  if (err != hipSuccess) return set_error(CA_ERR_HIP, "%s launch: %s", op, hipGetErrorString(err));
+  return CA_OK;
+}
+
+}  // extern "C"

@@ -28,6 +28,8 @@ from torch.nn import functional as F
 from . import _native
 from .ops import (SUPPORTED_HEAD_DIMS, _UNLIMITED_MODES, _bwd_qkv_workspace_bytes, _check_device,
                   _fwd_qkv_workspace_bytes, _mode, check_mode_limits, continuum_attention)
+from .paged import PagedCache, paged_attention, rotary_append
+from .rotary import Rotary
 
 _DTYPE_CODE = {torch.float32: _native.CA_DTYPE_F32, torch.bfloat16: _native.CA_DTYPE_BF16,
                torch.float16: _native.CA_DTYPE_F16}
@@ -519,6 +521,20 @@ class ContinuumSelfAttention(nn.Module):
         y = continuum_attention(q, k, v, self.log_qk_gain, self.ca_query_tile)
         return self.out(y.transpose(1, 2).reshape(Bsz, T, C))
 
+    def forward_cached(self, x, cache, layer, rotary):
+        """The layer for new tokens ``x [tokens, dim]`` whose room ``cache`` (a
+        PagedCache) has made: their keys and values are appended and the tokens
+        attend over everything cached."""
+        N, C = x.shape
+        q, k, v = self.qkv(x).to(cache.data.dtype).view(N, 3, self.heads, self.head_dim).unbind(1)
+        k_pages, v_pages = cache.k(layer), cache.v(layer)
+        q = rotary_append(q, k, v, cache.positions, rotary, k_pages, v_pages, cache.table, cache.lengths,
+                          cache.starts)
+        y = paged_attention(q, k_pages, v_pages, cache.table, cache.lengths, cache.starts, self.log_qk_gain,
+                            max_new=cache.max_new, max_length=max(cache.counts),
+                            weight_sums=None if cache.weight_sums is None else cache.weight_sums[layer])
+        return self.out(y.view(N, C).to(x.dtype))
+
 
 class GELUMLP(nn.Module):
     """fc1 -> tanh-GELU -> fc2 (cuda/continuum_attention.py:857-866)."""
@@ -598,6 +614,57 @@ class ContinuumDecoderLM(nn.Module):
             out["loss"] = F.cross_entropy(logits[:, :-1, :].reshape(-1, V), targets[:, 1:].reshape(-1),
                                           reduction="mean")
         return out
+
+    def make_cache(self, batch, max_length=None, dtype=None, **kw):
+        """A PagedCache for this decoder's layers: ``batch`` sequences of at most
+        ``max_length`` slots (default: block_size), in ``dtype`` (default: the
+        weights'); further arguments go to PagedCache."""
+        w = self.byte_emb.weight
+        return PagedCache(self.cfg.n_layers, batch, self.cfg.n_heads, self.cfg.d_model // self.cfg.n_heads,
+                          self.cfg.block_size if max_length is None else max_length,
+                          dtype=w.dtype if dtype is None else dtype, device=w.device, **kw)
+
+    # the positions of forward_cached; None: the training's (whole heads, neighbouring pairs, rope_theta)
+    rotary = None
+
+    @torch.no_grad()
+    def forward_cached(self, input_ids, cache, new=None):
+        """Logits ``[tokens, vocab]`` of new tokens, which are added to ``cache``
+        (make_cache): ``input_ids [B, n]``, n for every sequence, or ``[tokens]``
+        with ``new[b]`` of them for sequence b in turn.  A prompt in one piece or in
+        several, then its continuation token by token, gives the logits of
+        ``forward`` over the whole, up to rounding.  Set ``self.rotary`` for
+        contexts longer than the trained ones."""
+        if input_ids.dim() == 2 and new is None:
+            new = [input_ids.shape[1]] * input_ids.shape[0]
+        elif input_ids.dim() != 1 or new is None or sum(new) != input_ids.shape[0]:
+            raise ValueError("Input must be [B,T], or [tokens] with the sequences' counts in new")
+        if self.rotary is None or self.rotary.turns.device != cache.device:
+            if self.rotary is None:
+                self.rotary = Rotary(self.cfg.d_model // self.cfg.n_heads, self.cfg.rope_theta)
+            self.rotary = self.rotary.to(cache.device)
+        cache.extend(new)
+        x = self.byte_emb(input_ids.reshape(-1))
+        h = self.blocks[0].norm1(x)
+        for n, block in enumerate(self.blocks):
+            x, h = block.norm2.add_and_norm(x, block.attn.forward_cached(h, cache, n, self.rotary))
+            nxt = self.blocks[n + 1].norm1 if n + 1 < len(self.blocks) else self.norm_f
+            x, h = nxt.add_and_norm(x, block.mlp(h))
+        return self.lm_head(h)
+
+    @torch.no_grad()
+    def generate(self, input_ids, steps, cache=None):
+        """``[B, steps]`` tokens that continue ``input_ids [B, T]``, each the most
+        likely next one (of equal ones the first)."""
+        if cache is None:
+            cache = self.make_cache(input_ids.shape[0], input_ids.shape[1] + steps)
+        out = []
+        ids = input_ids
+        for _ in range(steps):
+            logits = self.forward_cached(ids, cache).view(*ids.shape, -1)[:, -1]
+            ids = logits.argmax(-1, keepdim=True)
+            out.append(ids)
+        return torch.cat(out, 1) if out else input_ids[:, :0]
 
     def parameter_breakdown(self):
         return {"byte_embedding": _numel(self.byte_emb), "decoder_blocks": _numel(self.blocks),

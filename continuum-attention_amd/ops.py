@@ -110,8 +110,13 @@ def _fwd_qkv_workspace_bytes(B: int, H: int, T: int, D: int) -> int:
     return int(_native.load().ca_fwd_qkv_workspace_bytes(B, H, T, D))
 
 
+_clear_hooks = []  # other modules' cached sizes
+
+
 def _clear_workspace_sizes() -> None:
     # the sizes follow the workspace cap and the split override
+    for f in _clear_hooks:
+        f()
     for f in (_fwd_workspace_bytes, _bwd_workspace_bytes, _fwd_op_workspace_bytes,
               _bwd_op_workspace_bytes, _fwd_qkv_workspace_bytes, _bwd_qkv_workspace_bytes):
         f.cache_clear()

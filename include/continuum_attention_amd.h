@@ -292,6 +292,94 @@ int ca_adamw_step(const ca_opt_tensor* tensors, int ntensors, const int* chunks,
 int ca_bf16_shadow(const ca_opt_tensor* tensors, int ntensors, const int* chunks, int nchunks,
                    void* stream);
 
+/* ---- Generation (no counterpart in the reference) ---------------------------
+ * A paged key/value cache of one attention layer.  Key head h of slot s of
+ * sequence b lies at  k + (table[b * table_stride + s / page_size] * page_stride
+ * + h * head_stride + s % page_size * row_stride)  elements, head_dim of them
+ * together; v alike.  lengths[b] counts the cached slots of sequence b with its
+ * new tokens; starts[b] .. starts[b + 1] are its new tokens among the token
+ * tensors' `tokens` rows (rows from starts[batch] on belong to no sequence and
+ * are left as they were).  Both are read on the device and held to what the
+ * table and the tokens have room for.  A table entry outside [0, num_pages) is
+ * never followed.  Rows are 16-byte aligned; head_dim is a multiple of 8 up to
+ * 128; a sequence has at most 2^30 slots. */
+typedef struct {
+  void* k;
+  void* v;
+  const int* table;
+  const int* lengths;
+  const int* starts;
+  long long page_stride, head_stride, row_stride, table_stride; /* elements */
+  int dtype, heads, head_dim, page_size, num_pages, pages_per_seq, batch, tokens;
+} ca_paged_cache;
+
+/* Continuum Attention of each sequence's new tokens over its cache: the token
+ * at slot p sees slots 0..p with the weights of the operator above, scores
+ * exp(log_gain[head]) / sqrt(head_dim) q.k.  q and out are token-major of
+ * cache->dtype, `heads` query heads (a multiple of the cache's; head i reads key
+ * head i / (heads / cache->heads)), with token and head strides in elements.
+ * sums, if given ([batch][cache->heads][sums_len] fp32 with batch and head
+ * strides): sums[b][h][s] += the weights slot s got from sequence b's new
+ * tokens, over the query heads of h.  max_new and max_length, the largest count
+ * of new tokens and cached length expected, size the grid and the workspace;
+ * other numbers on the device give the same results.  A token that sees nothing
+ * gets zeros; one that reads a table entry outside the cache gets NaN. */
+size_t ca_paged_attention_workspace_bytes(int batch, int kv_heads, int heads, int head_dim, int tokens,
+                                          int max_new, int max_length, int with_sums);
+int ca_paged_attention(const ca_paged_cache* cache, const void* q, long long q_token_stride,
+                       long long q_head_stride, int heads, const float* log_gain, void* out,
+                       long long out_token_stride, long long out_head_stride, float* sums,
+                       long long sums_batch_stride, long long sums_head_stride, int sums_len, int max_new,
+                       int max_length, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Of every sequence and key head keeps `budget` slots: the first `sinks`, the
+ * last `recent` and, of those between, the ones with the largest sums (of equal
+ * ones the first; NaN is the largest), all of them where there are no more, and
+ * copies their rows in order to slots 0, 1, .. of new_table's pages (of the same
+ * cache; pages no sequence still reads).  kept [batch][heads][budget] receives
+ * their former slots (-1 behind the last), new_sums (same shape) their sums (0
+ * behind), new_lengths [batch] the counts.  cache->starts is not read.
+ * new_table_stride * page_size must hold budget. */
+int ca_evict(const ca_paged_cache* cache, const float* sums, long long sums_batch_stride,
+             long long sums_head_stride, int sums_len, int budget, int sinks, int recent,
+             const int* new_table, long long new_table_stride, int* kept, float* new_sums,
+             int* new_lengths, void* stream);
+
+/* Rotary positions.  Pair p of a head's first rotary_dim dims turns by
+ * positions[token] * turns[p] full turns and is scaled by `magnitude`; pairs are
+ * dims (2p, 2p + 1) or, with `half`, (p, p + rotary_dim / 2); the other dims are
+ * copied.  inverse: turns back (the gradient).  q and k are token-major with
+ * token and head strides in elements; k may be NULL (k_heads 0), outputs may be
+ * the inputs.  positions are 32- or 64-bit integers (positions64). */
+typedef struct {
+  const void* q;
+  const void* k;
+  void* q_out;
+  void* k_out;
+  const void* positions;
+  const double* turns;
+  long long q_token_stride, q_head_stride, k_token_stride, k_head_stride;
+  long long q_out_token_stride, q_out_head_stride, k_out_token_stride, k_out_head_stride;
+  float magnitude;
+  int positions64, half, inverse, dtype, tokens, q_heads, k_heads, head_dim, rotary_dim;
+} ca_rotary;
+int ca_rotary_embedding(const ca_rotary* r, void* stream);
+/* The same for new tokens, with the rotated keys and the values v written to
+ * their slots of the cache (slot lengths[b] - new tokens of b + t) instead of
+ * k_out.  Slots without a page of the cache are left out. */
+int ca_rotary_append(const ca_rotary* r, const void* v, long long v_token_stride,
+                     long long v_head_stride, const ca_paged_cache* cache, void* stream);
+
+/* y[m][n] = sum_k x[m][k] scales[k / group][n] (code[n][k] - zeros[k / group][n]),
+ * zeros NULL: 8.  x, y, scales and zeros of `dtype`; rows of x and y x_stride and
+ * y_stride elements apart, scales and zeros [ceil(K / group)][N].  codes: [N] rows
+ * of ceil(K / 128) * 16 words of 32 bits, 16-byte aligned; word w holds columns
+ * 8w .. 8w + 7, column 8w + 2p in bits 4p and 8w + 2p + 1 in bits 16 + 4p.  group is
+ * 32, 64 or a multiple of 128.  An infinity in a row of x gives NaN there. */
+int ca_int4_linear(const void* x, long long x_stride, const unsigned* codes, const void* scales,
+                   const void* zeros, void* y, long long y_stride, int dtype, int M, int N, int K,
+                   int group, void* stream);
+
 /* ---- Diagnostics (no counterpart in the reference; used by bench.py) -------
  * Per-kernel timing with HIP events recorded on the launch stream around each
  * kernel launch of the calls above.  Kernel ids: 0 forward, 1 forward split
