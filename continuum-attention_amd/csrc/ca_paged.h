@@ -61,10 +61,13 @@ struct PagedAttnIO {
   long long sums_bs, sums_hs;
   int sums_len;
   int tokens, Hq, group;
-  int splits, split_keys;  // keys per split (a multiple of 30); the last takes the rest
+  int splits, split_keys;  // keys per split (a multiple of a tile's); the last takes the rest
   int row_tiles;           // row tiles of the grid; work groups walk the rest
+  // few rows: 2^row_log rows and tile_group tiles of 32 keys share a wave's 16
+  // columns; tile_group 0: many rows
+  int row_log, tile_group;
 };
-hipError_t launch_paged_attention(const PagedAttnIO& io, int dtype, int wave_rows, hipStream_t s);
+hipError_t launch_paged_attention(const PagedAttnIO& io, int dtype, hipStream_t s);
 hipError_t launch_paged_combine(const PagedAttnIO& io, int dtype, hipStream_t s);
 hipError_t launch_paged_sums(const PagedAttnIO& io, int dtype, int max_length, hipStream_t s);
 

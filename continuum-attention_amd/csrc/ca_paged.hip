@@ -27,9 +27,8 @@
 // instruction: the limb products of the training kernels cost as much time
 // once each wave has to split what it reads.
 //
-// Two shapes of a work group of four waves: up to 16 rows per key head (single
-// tokens) all waves hold the same rows and take tiles in turn, each with V of
-// its own; more rows are dealt to the waves, which share V.
+// Few rows (up to 16 per key head: single tokens) have a kernel of their own
+// (ca_paged_few_kernel).
 #include "ca_paged.h"
 
 namespace ca {
@@ -158,9 +157,8 @@ __device__ __forceinline__ void load_k(const PagedCache& c, const E* kh, const R
 }
 // Scores q . k of the lane's query and its eight slots, unscaled.
 template <class E, int DT>
-__device__ __forceinline__ void tile_products(const KRows<E, DT>& kr, const Rows<E, DT>& R, float (&s)[8]) {
+__device__ __forceinline__ void add_products(const KRows<E, DT>& kr, const Rows<E, DT>& R, f32x4 (&acc)[2]) {
   typedef Tile<E, DT> P;
-  f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
   for (int p = 0; p < P::kPieces; ++p) {
     if constexpr (P::kF32) {
@@ -176,6 +174,11 @@ __device__ __forceinline__ void tile_products(const KRows<E, DT>& kr, const Rows
       acc[1] = mfma16_of(kr.k[1][p], R.q[p], acc[1], (const E*)nullptr);
     }
   }
+}
+template <class E, int DT>
+__device__ __forceinline__ void tile_products(const KRows<E, DT>& kr, const Rows<E, DT>& R, float (&s)[8]) {
+  f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+  add_products<E, DT>(kr, R, acc);
 #pragma unroll
   for (int r = 0; r < 8; ++r) s[r] = acc[r >> 2][r & 3];
 }
@@ -220,6 +223,38 @@ __device__ __forceinline__ void tile_weights(const float (&s)[8], int key0, int 
   w[7] = G4 == 3 ? 0.f : w[7];
 }
 
+// The same where the lane's eight keys have neighbours on both sides (sl, sr,
+// relative like s): every key is the lane's own.
+template <bool MASK>
+__device__ __forceinline__ void span_weights(const float (&s)[8], float sl, float s_end, int key0, int pos,
+                                             float (&w)[8]) {
+  float pl = fast_exp2(sl);
+#pragma unroll
+  for (int r = 0; r < 9; ++r) {
+    const float sr = r < 8 ? s[r] : s_end;
+    const float pr = fast_exp2(sr);
+    float L, R;
+    seg_shares(sl, sr, pl, pr, L, R);
+    const int key = key0 + r;
+    if (MASK) {
+      const bool ok = key >= 1 && key <= pos;
+      L = ok ? L : 0.f;
+      R = ok ? R : 0.f;
+    }
+    if (r > 0) w[r - 1] += L;
+    if (r < 8) {
+      w[r] = R;
+      if (MASK) {
+        const float cap = 2.0f * pr;
+        w[r] += key == 0 && pos >= 0 ? cap : 0.f;
+        w[r] += key == pos && pos >= 0 ? cap : 0.f;
+      }
+    }
+    sl = sr;
+    pl = pr;
+  }
+}
+
 // One wave's running softmax: shift (log2 units, whole), sum of weights (this
 // lane's part) and O^T, whose lane holds columns 16 b + 4 G4 + e of its query.
 template <int DT> struct Running {
@@ -257,10 +292,37 @@ __device__ __forceinline__ u32x4 finite_part(u32x4 x) {
 }
 __device__ __forceinline__ bool is_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 
-// O^T += V^T W^T over the tile's 32 slots; vs: the tile's V rows.  FINITE:
-// without the values that are not finite.
+// Weights in two 16-bit limbs, as an operand.
+template <class E> struct Limbs16 {
+  u32x4 hi, lo;
+};
+template <class E>
+__device__ __forceinline__ Limbs16<E> limbs16(const float (&w)[8]) {
+  Limbs16<E> r;
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    const float a = w[2 * p], b = w[2 * p + 1];
+    if constexpr (std::is_same<E, __bf16>::value) {
+      unsigned x[3];
+      split_pair_limbs<2>(a, b, x);
+      r.hi[p] = x[0];
+      r.lo[p] = x[1];
+    } else {
+      typedef __fp16 h2 __attribute__((ext_vector_type(2)));
+      const h2 h = __builtin_amdgcn_cvt_pkrtz(a, b);
+      const h2 l = __builtin_amdgcn_cvt_pkrtz(a - (float)h[0], b - (float)h[1]);
+      r.hi[p] = __builtin_bit_cast(unsigned, h);
+      r.lo[p] = __builtin_bit_cast(unsigned, l);
+    }
+  }
+  return r;
+}
+
+// O^T += V^T W^T over the tile's 32 slots; vs: the tile's V rows; the weights as
+// they are (fp32) or in limbs.  FINITE: without the values that are not finite.
 template <class E, int DT, bool FINITE>
-__device__ __forceinline__ void add_values(Running<DT>& st, const E* vs, const float (&w)[8]) {
+__device__ __forceinline__ void add_values(Running<DT>& st, const E* vs, const float (&w)[8],
+                                           const Limbs16<E>& wl) {
   typedef Tile<E, DT> P;
   const int lane = threadIdx.x & 63, i = lane & 15, G4 = lane >> 4;
   if constexpr (P::kF32) {
@@ -278,31 +340,14 @@ __device__ __forceinline__ void add_values(Running<DT>& st, const E* vs, const f
       st.o[b] += part;
     }
   } else {
-    u32x4 hi, lo;
-#pragma unroll
-    for (int p = 0; p < 4; ++p) {
-      const float a = w[2 * p], b = w[2 * p + 1];
-      if constexpr (std::is_same<E, __bf16>::value) {
-        unsigned x[3];
-        split_pair_limbs<2>(a, b, x);
-        hi[p] = x[0];
-        lo[p] = x[1];
-      } else {
-        typedef __fp16 h2 __attribute__((ext_vector_type(2)));
-        const h2 h = __builtin_amdgcn_cvt_pkrtz(a, b);
-        const h2 l = __builtin_amdgcn_cvt_pkrtz(a - (float)h[0], b - (float)h[1]);
-        hi[p] = __builtin_bit_cast(unsigned, h);
-        lo[p] = __builtin_bit_cast(unsigned, l);
-      }
-    }
     // transposed reads: see lds_read_tr8
     const __bf16* base = reinterpret_cast<const __bf16*>(vs) + (8 * G4 + (i >> 2)) * P::kRow + 4 * (i & 3);
 #pragma unroll
     for (int b = 0; b < DT / 16; ++b) {
       u32x4 a = __builtin_bit_cast(u32x4, lds_read_tr8(base + 16 * b, base + 4 * P::kRow + 16 * b));
       if (FINITE) a = finite_part<E>(a);
-      st.o[b] = mfma16_of(a, lo, st.o[b], (const E*)nullptr);
-      st.o[b] = mfma16_of(a, hi, st.o[b], (const E*)nullptr);
+      st.o[b] = mfma16_of(a, wl.lo, st.o[b], (const E*)nullptr);
+      st.o[b] = mfma16_of(a, wl.hi, st.o[b], (const E*)nullptr);
     }
   }
 }
@@ -312,7 +357,7 @@ __device__ __forceinline__ void add_values(Running<DT>& st, const E* vs, const f
 // would be with any other values there, bit for bit.
 template <class E, int DT>
 __device__ __forceinline__ void add_values_seen(Running<DT>& st, const E* vs, const float (&w)[8], int tile_key,
-                                                int pos) {
+                                                int pos, int first_slot, int end_slot) {
   typedef Tile<E, DT> P;
   const int lane = threadIdx.x & 63, i = lane & 15, G4 = lane >> 4;
 #pragma unroll
@@ -320,7 +365,7 @@ __device__ __forceinline__ void add_values_seen(Running<DT>& st, const E* vs, co
     for (int g = 0; g < 4; ++g) {
       const int slot = 8 * g + r;
       const float x = __shfl(w[r], 16 * g + i);
-      const bool seen = slot > 0 && slot < 31 && tile_key + slot <= pos;
+      const bool seen = slot >= first_slot && slot < end_slot && tile_key + slot <= pos;
 #pragma unroll
       for (int b = 0; b < DT / 16; ++b) {
         const f32x4 v = ld4(vs + slot * P::kRow + 16 * b + 4 * G4);
@@ -342,18 +387,15 @@ __device__ __forceinline__ bool bad_pages(const PagedCache& c, const int* table,
   return __syncthreads_or(bad);
 }
 
-// WR: waves that hold different rows (4), or 1: the four waves hold the same 16
-// rows and take tiles in turn.
-template <class E, int DT, int WR>
+// Many rows: four waves of 16 rows each share the tiles of V, which they stage
+// two in turn.
+template <class E, int DT>
 __global__ __launch_bounds__(256) void ca_paged_attention_kernel(PagedAttnIO io) {
   typedef Tile<E, DT> P;
-  constexpr int kStage = 64 * WR;                                     // threads that stage a tile of V
-  constexpr int kV = (32 * P::kChunks + kStage - 1) / kStage;         // 16-byte loads of each
-  constexpr int kBufs = WR == 1 ? 4 : 2;                              // one per wave, or two in turn
-  constexpr int kVBytes = kBufs * 32 * P::kRow * (int)sizeof(E);
-  constexpr int kJoinBytes = WR == 1 ? 4 * 16 * (DT + 4) * (int)sizeof(float) : 0;
-  __shared__ __attribute__((aligned(16))) unsigned char lds[kVBytes > kJoinBytes ? kVBytes : kJoinBytes];
-  __shared__ int special[kBufs];  // tile (plus one) whose V holds a value that is not finite
+  constexpr int kRows = 64;
+  constexpr int kV = (32 * P::kChunks + 255) / 256;  // 16-byte loads of a thread per tile of V
+  __shared__ __attribute__((aligned(16))) E vbuf[2 * 32 * P::kRow];
+  __shared__ int special[2];  // tile (plus one) whose V holds a value that is not finite
 
   const PagedCache& c = io.c;
   const int tid = threadIdx.x, lane = tid & 63, i16 = lane & 15, G4 = lane >> 4;
@@ -369,12 +411,12 @@ __global__ __launch_bounds__(256) void ca_paged_attention_kernel(PagedAttnIO io)
   const int* table = c.table + (long long)b * c.table_stride;
   const E* kh = static_cast<const E*>(c.k) + (long long)h * c.head_stride;
   const E* vh = static_cast<const E*>(c.v) + (long long)h * c.head_stride;
-  const int tiles = (rows + 16 * WR - 1) / (16 * WR);
+  const int tiles = (rows + kRows - 1) / kRows;
 
   // longest rows first
   for (int back = tile0; back < tiles; back += io.row_tiles) {
-    const int row0 = (tiles - 1 - back) * 16 * WR;
-    const int last_row = row0 + 16 * WR < rows ? row0 + 16 * WR - 1 : rows - 1;
+    const int row0 = (tiles - 1 - back) * kRows;
+    const int last_row = row0 + kRows < rows ? row0 + kRows - 1 : rows - 1;
     const int pos_max = sp.len - sp.n + last_row / io.group;  // last slot any row sees
     const int pos_min = sp.len - sp.n + row0 / io.group;
     const int first = split * io.split_keys;
@@ -383,13 +425,13 @@ __global__ __launch_bounds__(256) void ca_paged_attention_kernel(PagedAttnIO io)
     }
     const int end = split == io.splits - 1 ? pos_max + 1
                     : first + io.split_keys < pos_max + 1 ? first + io.split_keys : pos_max + 1;
-    const Rows<E, DT> R = load_rows<E, DT>(io, sp, h, row0 + (WR == 1 ? 0 : 16 * wave) + i16);
+    const Rows<E, DT> R = load_rows<E, DT>(io, sp, h, row0 + 16 * wave + i16);
     Running<DT> st;
     st.m = kNegBig;
     st.z = 0.f;
 #pragma unroll
     for (int x = 0; x < DT / 16; ++x) st.o[x] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (tid < kBufs) special[tid] = 0;
+    if (tid < 2) special[tid] = 0;
     const int ntiles = end > first ? (end - first + kOwned - 1) / kOwned : 0;
     bool bad = false;
     if (ntiles > 0) {
@@ -401,26 +443,22 @@ __global__ __launch_bounds__(256) void ca_paged_attention_kernel(PagedAttnIO io)
     if (bad) {
       st.m = st.z = nan_value();
     } else {
-      constexpr int kStep = WR == 1 ? 4 : 1;  // tiles between a wave's
-      const int t_first = WR == 1 ? wave : 0;
-      E* vbuf = reinterpret_cast<E*>(lds);
       KRows<E, DT> kr;
       RowRef kref[2], vref[kV];
       u32x4 vreg[kV];
-      const int stage_id = WR == 1 ? lane : tid;
       auto refs = [&](int t) {  // page numbers of tile t's rows
         const int key = first + t * kOwned - 1;
 #pragma unroll
         for (int x = 0; x < 2; ++x) kref[x] = row_ref(c, table, key + k_slot(x), pos_max);
 #pragma unroll
         for (int x = 0; x < kV; ++x)
-          vref[x] = row_ref(c, table, key + (stage_id + x * kStage) / P::kChunks, pos_max);
+          vref[x] = row_ref(c, table, key + (tid + x * 256) / P::kChunks, pos_max);
       };
       auto load_v = [&](int t) {
         const int key = first + t * kOwned - 1;
 #pragma unroll
         for (int x = 0; x < kV; ++x) {
-          const int u = stage_id + x * kStage, row = u / P::kChunks, d = u % P::kChunks * P::kVec;
+          const int u = tid + x * 256, row = u / P::kChunks, d = u % P::kChunks * P::kVec;
           // rows of other tiles and behind the last key stay out: zeros
           const bool mine = row > 0 && row < 31 && key + row < end && d < c.D;
           vreg[x] = mine ? *reinterpret_cast<const u32x4*>(vh + row_at(c, vref[x]) + d) : u32x4{0, 0, 0, 0};
@@ -430,33 +468,30 @@ __global__ __launch_bounds__(256) void ca_paged_attention_kernel(PagedAttnIO io)
         const bool look = first + t * kOwned + 30 > pos_min;
 #pragma unroll
         for (int x = 0; x < kV; ++x) {
-          const int u = stage_id + x * kStage, row = u / P::kChunks, d = u % P::kChunks * P::kVec;
-          if ((32 * P::kChunks) % kStage == 0 || row < 32) {
+          const int u = tid + x * 256, row = u / P::kChunks, d = u % P::kChunks * P::kVec;
+          if ((32 * P::kChunks) % 256 == 0 || row < 32) {
             *reinterpret_cast<u32x4*>(vbuf + (buf * 32 + row) * P::kRow + d) = vreg[x];
             if (look && any_special(vreg[x], (const E*)nullptr)) special[buf] = t + 1;
           }
         }
       };
-      auto sync = [&]() {
-        if constexpr (WR == 1) wave_lds_sync(); else __syncthreads();
-      };
-      if (t_first < ntiles) {
-        refs(t_first);
+      if (ntiles > 0) {
+        refs(0);
         load_k<E, DT>(c, kh, kref, kr);
-        load_v(t_first);
-        refs(t_first + kStep);
-        store_v(t_first, WR == 1 ? wave : 0);
-        sync();
+        load_v(0);
+        refs(1);
+        store_v(0, 0);
+        __syncthreads();
       }
-      for (int t = t_first; t < ntiles; t += kStep) {
-        const int buf = WR == 1 ? wave : t & 1;
+      for (int t = 0; t < ntiles; ++t) {
+        const int buf = t & 1;
         const int key = first + t * kOwned - 1;  // key of slot 0
         float s[8], w[8];
         tile_products<E, DT>(kr, R, s);
-        if (t + kStep < ntiles) {
+        if (t + 1 < ntiles) {
           load_k<E, DT>(c, kh, kref, kr);
-          load_v(t + kStep);
-          refs(t + 2 * kStep);
+          load_v(t + 1);
+          refs(t + 2);
         }
         const int key0 = key + 8 * G4;
         const bool mask = key < 0 || key + 31 > pos_min;
@@ -484,22 +519,314 @@ __global__ __launch_bounds__(256) void ca_paged_attention_kernel(PagedAttnIO io)
 #pragma unroll
         for (int r = 0; r < 8; ++r) st.z += w[r];
         const E* vs = vbuf + buf * 32 * P::kRow;
+        Limbs16<E> wl;
+        if constexpr (!P::kF32) wl = limbs16<E>(w);
         if (mask && special[buf] == t + 1) {
-          add_values<E, DT, true>(st, vs, w);
-          add_values_seen<E, DT>(st, vs, w, key, R.pos);
+          add_values<E, DT, true>(st, vs, w, wl);
+          add_values_seen<E, DT>(st, vs, w, key, R.pos, 1, 31);
         } else {
-          add_values<E, DT, false>(st, vs, w);
+          add_values<E, DT, false>(st, vs, w, wl);
         }
-        if (t + kStep < ntiles) store_v(t + kStep, WR == 1 ? wave : buf ^ 1);
-        sync();
+        if (t + 1 < ntiles) store_v(t + 1, buf ^ 1);
+        __syncthreads();
       }
       st.z = rows_sum(st.z);
     }
 
     const long long nrows = (long long)io.tokens * io.Hq;
-    if constexpr (WR == 1) {
-      // join the four waves' parts; row_bytes: O, then m and z
-      constexpr int kJRow = DT + 4;
+    {
+      const float meff = st.m - weight_octaves<E>();
+      if (R.row >= 0) {
+        if (io.splits == 1) {
+          const float inv = st.z == 0.f ? 0.f : 1.0f / st.z;
+          const int r = row0 + 16 * wave + i16, t = r / io.group, head = h * io.group + r - t * io.group;
+          E* o = static_cast<E*>(io.out) + (long long)(sp.t0 + t) * io.o_ts + (long long)head * io.o_hs;
+#pragma unroll
+          for (int x = 0; x < DT / 16; ++x)
+            if (16 * x + 4 * G4 < c.D) st4(o + 16 * x + 4 * G4, st.o[x] * inv);
+          if (io.stats && G4 == 0) {
+            io.stats[2 * R.row] = meff;
+            io.stats[2 * R.row + 1] = inv;
+          }
+        } else {
+          float* o = io.part_o + (split * nrows + R.row) * c.D;
+#pragma unroll
+          for (int x = 0; x < DT / 16; ++x)
+            if (16 * x + 4 * G4 < c.D) st4(o + 16 * x + 4 * G4, st.o[x]);
+          if (G4 == 0) {
+            io.part_ml[2 * (split * nrows + R.row)] = meff;
+            io.part_ml[2 * (split * nrows + R.row) + 1] = st.z;
+          }
+        }
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// Few rows: up to 16 per key head.  One token of one head would leave 15 of a
+// tile's 16 columns empty, and the segment math is the longest part of a tile, so
+// the columns hold RP = 2^row_log rows times TP tiles of 32 keys: column c is row
+// c % RP over tile c / RP of a group of TP tiles.  The group's scores come from TP
+// products into one accumulator, each with the queries zeroed outside its tile's
+// columns; the segments are then formed once for all of the group; and O^T
+// takes TP products again, each with the weights of its own columns.  Every
+// column keeps its own running maximum, and columns and waves are joined at the
+// end.  Per tile this leaves some 60 vector instructions of 520 with one tile at
+// a time, so that the bytes bound it.
+//
+// Tiles here own all of their 32 keys: neighbours are other columns' scores, and
+// the two beyond the group come from one more product (K rows k0 - 1 and k0 + 32 TP).
+// So tiles start at multiples of 32, and where pages do too (PAGE32) a tile lies
+// in one page: its number is read once for the wave and addresses are a scalar
+// base and a constant offset per lane.
+template <class E, int DT> struct Few {
+  typedef Tile<E, DT> P;
+  static constexpr int kV = 32 * P::kChunks / 64;  // 16-byte pieces of V of a lane per tile
+};
+template <class E, int DT> struct VRows {
+  u32x4 v[Few<E, DT>::kV];
+};
+
+template <class E, int DT, bool PAGE32>
+__global__ __launch_bounds__(256) void ca_paged_few_kernel(PagedAttnIO io) {
+  typedef Tile<E, DT> P;
+  constexpr int kV = Few<E, DT>::kV;
+  constexpr int kVBytes = 4 * 32 * P::kRow * (int)sizeof(E);
+  constexpr int kJRow = DT + 4;
+  constexpr int kJoinBytes = 4 * 16 * kJRow * (int)sizeof(float);
+  __shared__ __attribute__((aligned(16))) unsigned char lds[kVBytes > kJoinBytes ? kVBytes : kJoinBytes];
+
+  const PagedCache& c = io.c;
+  const int tid = threadIdx.x, lane = tid & 63, i16 = lane & 15, G4 = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int slices = c.batch * c.heads;
+  const int slice = blockIdx.x % slices, rest = blockIdx.x / slices;
+  const int split = rest % io.splits, tile0 = rest / io.splits;
+  const int b = slice / c.heads, h = slice - b * c.heads;
+  const SeqSpan sp = seq_span(c, b, io.tokens);
+  const int rows = sp.n * io.group;
+  const int* table = c.table + (long long)b * c.table_stride;
+  const E* kh = static_cast<const E*>(c.k) + (long long)h * c.head_stride;
+  const E* vh = static_cast<const E*>(c.v) + (long long)h * c.head_stride;
+  const int RP = 1 << io.row_log, TP = io.tile_group;
+  const int row_tiles = (rows + RP - 1) >> io.row_log;
+  const int u_col = i16 >> io.row_log;  // the tile of this lane's column
+  const int k_d = DT / 4 * G4;          // first of the lane's D values of K
+  E* vs = reinterpret_cast<E*>(lds) + wave * 32 * P::kRow;
+
+  for (int back = tile0; back < row_tiles; back += io.row_tiles) {
+    const int row0 = (row_tiles - 1 - back) << io.row_log;
+    const int last_row = row0 + RP < rows ? row0 + RP - 1 : rows - 1;
+    const int pos_max = sp.len - sp.n + last_row / io.group;
+    const int pos_min = sp.len - sp.n + row0 / io.group;
+    const int first = split * io.split_keys;
+    if (pos_max < first && split > 0) continue;  // the join knows
+    const int end = split == io.splits - 1 || first + io.split_keys > pos_max ? pos_max + 1 : first + io.split_keys;
+    const Rows<E, DT> R = load_rows<E, DT>(io, sp, h, row0 + (i16 & (RP - 1)));
+    Running<DT> st;
+    st.m = kNegBig;
+    st.z = 0.f;
+#pragma unroll
+    for (int x = 0; x < DT / 16; ++x) st.o[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+    bool bad = false;
+    if (end > first) bad = bad_pages(c, table, first > 0 ? first - 1 : 0, end <= pos_max ? end : pos_max);
+    if (bad) {
+      st.m = st.z = nan_value();
+    } else {
+      const int step = 32 * TP;
+      // Page numbers of a group: lane u < 16 tile u's, lanes 16 and 17 the
+      // neighbours'.  (Only what PAGE32 needs.)
+      auto group_pages = [&](int k0) {
+        int key = lane < 16 ? k0 + 32 * lane : lane == 16 ? k0 - 1 : k0 + step;
+        key = key < 0 ? 0 : key > pos_max ? pos_max : key;
+        return table[page_of(c.div, key)];
+      };
+      int ids = 0, next_ids = 0;
+      auto tile_base = [&](int key, int u) {  // of a tile in one page
+        const int idx = page_of(c.div, key);
+        const int page = __builtin_amdgcn_readlane(ids, u);
+        return (long long)page * c.page_stride + (long long)(key - idx * (int)c.div.size) * c.row_stride;
+      };
+      auto load_ktile = [&](int key, int u, KRows<E, DT>& out) {
+        if constexpr (PAGE32) {
+          const E* base = kh + tile_base(key, u);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int off = k_slot(x) * (int)c.row_stride + k_d;
+#pragma unroll
+            for (int j = 0; j < P::kPieces; ++j)
+              out.k[x][j] = k_d + P::kVec * j < c.D ? *reinterpret_cast<const u32x4*>(base + off + P::kVec * j)
+                                                    : u32x4{0, 0, 0, 0};
+          }
+        } else {
+          RowRef ref[2];
+#pragma unroll
+          for (int x = 0; x < 2; ++x) ref[x] = row_ref(c, table, key + k_slot(x), pos_max);
+          load_k<E, DT>(c, kh, ref, out);
+        }
+      };
+      auto load_vtile = [&](int key, int u, VRows<E, DT>& out) {
+        const E* base = vh;
+        if constexpr (PAGE32) base += tile_base(key, u);
+        const bool whole = key + 32 <= end;
+#pragma unroll
+        for (int x = 0; x < kV; ++x) {
+          const int at = lane + 64 * x, row = at / P::kChunks, d = at % P::kChunks * P::kVec;
+          const bool mine = d < c.D && (whole || key + row < end);  // behind the last key: zeros
+          if constexpr (PAGE32) {
+            out.v[x] = mine ? *reinterpret_cast<const u32x4*>(base + (row * (int)c.row_stride + d)) : u32x4{0, 0, 0, 0};
+          } else {
+            const RowRef ref = row_ref(c, table, key + row, pos_max);
+            out.v[x] = mine ? *reinterpret_cast<const u32x4*>(base + row_at(c, ref) + d) : u32x4{0, 0, 0, 0};
+          }
+        }
+      };
+      int k0 = first + wave * step;
+      if (PAGE32 && k0 < end) ids = group_pages(k0);
+      for (; k0 < end; k0 += 4 * step) {
+        const int n = (end - k0 + 31) / 32 < TP ? (end - k0 + 31) / 32 : TP;  // tiles of this group
+        if (PAGE32 && k0 + 4 * step < end) next_ids = group_pages(k0 + 4 * step);
+        // scores of the group, and of its two neighbours
+        KRows<E, DT> ka, kb;
+        u32x4 kn[P::kPieces];
+        load_ktile(k0, 0, ka);
+        {
+          int key = i16 == 1 ? k0 + step : k0 - 1;
+          key = key < 0 ? 0 : key > pos_max ? pos_max : key;
+          RowRef ref;
+          if constexpr (PAGE32) {
+            const int idx = page_of(c.div, key);
+            const int left = __builtin_amdgcn_readlane(ids, 16), right = __builtin_amdgcn_readlane(ids, 17);
+            ref = RowRef{i16 == 1 ? right : left, key - idx * (int)c.div.size};
+          } else {
+            ref = row_ref(c, table, key, pos_max);
+          }
+          const E* p = kh + row_at(c, ref) + k_d;
+#pragma unroll
+          for (int j = 0; j < P::kPieces; ++j)
+            kn[j] = k_d + P::kVec * j < c.D ? *reinterpret_cast<const u32x4*>(p + P::kVec * j) : u32x4{0, 0, 0, 0};
+        }
+        f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+        auto products = [&](const KRows<E, DT>& kr, int u) {
+          Rows<E, DT> Q = R;
+          if (TP > 1) {
+#pragma unroll
+            for (int p = 0; p < P::kPieces; ++p)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) Q.q[p][e] = u_col == u ? Q.q[p][e] : 0u;
+          }
+          add_products<E, DT>(kr, Q, acc);
+        };
+        for (int u = 0; u < n; u += 2) {
+          if (u + 1 < n) load_ktile(k0 + 32 * (u + 1), u + 1, kb);
+          products(ka, u);
+          if (u + 2 < n) load_ktile(k0 + 32 * (u + 2), u + 2, ka);
+          if (u + 1 < n) products(kb, u + 1);
+        }
+        VRows<E, DT> v;
+        load_vtile(k0, 0, v);
+        f32x4 beyond = f32x4{0.f, 0.f, 0.f, 0.f};  // lane row 0: left, right
+#pragma unroll
+        for (int p = 0; p < P::kPieces; ++p) {
+          if constexpr (P::kF32) {
+            const f32x4 a = __builtin_bit_cast(f32x4, kn[p]), q = __builtin_bit_cast(f32x4, R.q[p]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) beyond = mfma16_f32(a[e], q[e], beyond);
+          } else {
+            beyond = mfma16_of(kn[p], R.q[p], beyond, (const E*)nullptr);
+          }
+        }
+        float s[8], w[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) s[r] = acc[r >> 2][r & 3] * R.scale;
+        const int key0 = k0 + 32 * u_col + 8 * G4;
+        const bool mask = k0 == 0 || k0 + step > pos_min;
+        float mt = kNegBig;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) mt = fmaxf(mt, !mask || key0 + r <= R.pos ? s[r] : kNegBig);
+        mt = rows_max(mt);
+        const bool grow = mt > st.m + kLazyRescale;
+        if (wave_any(grow)) {
+          const float m = grow ? rintf(mt) : st.m;
+          const float alpha = grow ? fast_exp2(st.m - m) : 1.0f;
+#pragma unroll
+          for (int x = 0; x < DT / 16; ++x) st.o[x] *= alpha;
+          st.z *= alpha;
+          st.m = m;
+        }
+        // neighbours: the lane rows before and behind; past a tile's ends the
+        // next columns' and past the group's the two products'
+        float s_left = s[7], s_right = s[0];
+        if (TP > 1) {
+          s_left = __shfl(s[7], (lane & 48) | ((i16 - RP) & 15));
+          s_right = __shfl(s[0], (lane & 48) | ((i16 + RP) & 15));
+        }
+        s_right = u_col == TP - 1 ? beyond[1] * R.scale : s_right;
+        s_left = row_before(G4 == 3 ? s_left : s[7]);
+        s_left = G4 == 0 && u_col == 0 ? beyond[0] * R.scale : s_left;
+        s_right = row_behind(G4 == 0 ? s_right : s[0]);
+        const float shift = st.m + (kShareShift - weight_octaves<E>());
+#pragma unroll
+        for (int r = 0; r < 8; ++r) s[r] -= shift;
+        if (mask) span_weights<true>(s, s_left - shift, s_right - shift, key0, R.pos, w);
+        else span_weights<false>(s, s_left - shift, s_right - shift, key0, R.pos, w);
+#pragma unroll
+        for (int r = 0; r < 8; ++r) st.z += w[r];
+        Limbs16<E> wl;
+        if constexpr (!P::kF32) wl = limbs16<E>(w);
+        for (int u = 0; u < n; ++u) {
+          bool special = false;
+          const bool look = k0 + 32 * (u + 1) > pos_min;
+#pragma unroll
+          for (int x = 0; x < kV; ++x) {
+            const int at = lane + 64 * x, row = at / P::kChunks, d = at % P::kChunks * P::kVec;
+            *reinterpret_cast<u32x4*>(vs + row * P::kRow + d) = v.v[x];
+            if (look) special = special || any_special(v.v[x], (const E*)nullptr);
+          }
+          wave_lds_sync();
+          if (u + 1 < n) load_vtile(k0 + 32 * (u + 1), u + 1, v);
+          const bool mine = TP == 1 || u_col == u;
+          float wu[8];
+          Limbs16<E> lu = wl;
+          if constexpr (P::kF32) {
+#pragma unroll
+            for (int r = 0; r < 8; ++r) wu[r] = mine ? w[r] : 0.f;
+          } else if (TP > 1) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              lu.hi[e] = mine ? wl.hi[e] : 0u;
+              lu.lo[e] = mine ? wl.lo[e] : 0u;
+            }
+          }
+          if (look && wave_any(special)) {
+            add_values<E, DT, true>(st, vs, wu, lu);
+            add_values_seen<E, DT>(st, vs, w, k0 + 32 * u, mine ? R.pos : -1, 0, 32);
+          } else {
+            add_values<E, DT, false>(st, vs, wu, lu);
+          }
+          wave_lds_sync();
+        }
+        ids = next_ids;
+      }
+      st.z = rows_sum(st.z);
+      // columns of one row
+      for (int x = RP; x < RP * TP; x <<= 1) {
+        const float pm = __shfl_xor(st.m, x), pz = __shfl_xor(st.z, x);
+        const float m = fmaxf(st.m, pm);
+        const float a = fast_exp2(st.m - m), e = fast_exp2(pm - m);
+#pragma unroll
+        for (int y = 0; y < DT / 16; ++y)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) st.o[y][q] = st.o[y][q] * a + __shfl_xor(st.o[y][q], x) * e;
+        st.z = st.z * a + pz * e;
+        st.m = m;
+      }
+    }
+
+    const long long nrows = (long long)io.tokens * io.Hq;
+    {
+      // join the four waves' parts: O, then m and z
       float* join = reinterpret_cast<float*>(lds);
       __syncthreads();
       {
@@ -513,7 +840,7 @@ __global__ __launch_bounds__(256) void ca_paged_attention_kernel(PagedAttnIO io)
       }
       __syncthreads();
       constexpr int kQuads = DT / 4;
-      for (int u = tid; u < 16 * kQuads; u += 256) {
+      for (int u = tid; u < RP * kQuads; u += 256) {
         const int r = u / kQuads, d = u % kQuads * 4;
         const int rr = row0 + r;
         if (rr >= rows || d >= c.D) continue;
@@ -547,53 +874,31 @@ __global__ __launch_bounds__(256) void ca_paged_attention_kernel(PagedAttnIO io)
         }
       }
       __syncthreads();  // the next row tile stages V over it
-    } else {
-      const float meff = st.m - weight_octaves<E>();
-      if (R.row >= 0) {
-        if (io.splits == 1) {
-          const float inv = st.z == 0.f ? 0.f : 1.0f / st.z;
-          const int r = row0 + 16 * wave + i16, t = r / io.group, head = h * io.group + r - t * io.group;
-          E* o = static_cast<E*>(io.out) + (long long)(sp.t0 + t) * io.o_ts + (long long)head * io.o_hs;
-#pragma unroll
-          for (int x = 0; x < DT / 16; ++x)
-            if (16 * x + 4 * G4 < c.D) st4(o + 16 * x + 4 * G4, st.o[x] * inv);
-          if (io.stats && G4 == 0) {
-            io.stats[2 * R.row] = meff;
-            io.stats[2 * R.row + 1] = inv;
-          }
-        } else {
-          float* o = io.part_o + (split * nrows + R.row) * c.D;
-#pragma unroll
-          for (int x = 0; x < DT / 16; ++x)
-            if (16 * x + 4 * G4 < c.D) st4(o + 16 * x + 4 * G4, st.o[x]);
-          if (G4 == 0) {
-            io.part_ml[2 * (split * nrows + R.row)] = meff;
-            io.part_ml[2 * (split * nrows + R.row) + 1] = st.z;
-          }
-        }
-      }
-      __syncthreads();
     }
   }
 }
 
-// Joins the splits of a row: one wave per row, DT / 4 lanes over its columns and
-// the remaining factor of 64 over the splits.
-template <class E, int DT>
+// Joins the splits of a row: DT / 4 lanes over its columns and the remaining
+// factor of 64 over the splits, WPR waves per row (four where there are many
+// splits, as for few rows: 64 splits of 16 rows took 9.6 us with one wave).
+template <class E, int DT, int WPR>
 __global__ __launch_bounds__(256) void ca_paged_combine_kernel(PagedAttnIO io) {
-  constexpr int kQuads = DT / 4, kLanes = 64 / kQuads;
+  constexpr int kQuads = DT / 4, kLanes = 64 / kQuads, kRows = 4 / WPR;
+  __shared__ float join[WPR == 1 ? 1 : 4][DT + 4];
   const PagedCache& c = io.c;
   const int slices = c.batch * c.heads;
   const int slice = blockIdx.x % slices, part = blockIdx.x / slices;
   const int b = slice / c.heads, h = slice - b * c.heads;
   const SeqSpan sp = seq_span(c, b, io.tokens);
-  const int rows = sp.n * io.group, lane = threadIdx.x & 63;
-  const int d = lane % kQuads * 4, sub = lane / kQuads;
+  const int rows = sp.n * io.group, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int d = lane % kQuads * 4, sub = lane / kQuads + (WPR == 1 ? 0 : wave * kLanes);
   const long long nrows = (long long)io.tokens * io.Hq;
   const int parts = gridDim.x / slices;
   // every work group of the attention kernel wrote the rows of its tile up to
   // the last slot any of them sees: a row's splits are those up to its own slot
-  for (int r = part * 4 + (threadIdx.x >> 6); r < rows; r += 4 * parts) {
+  for (int r0 = part * kRows; r0 < rows; r0 += kRows * parts) {
+    const int r = r0 + (WPR == 1 ? wave : 0);
+    if (WPR == 1 && r >= rows) continue;
     const int t = r / io.group, head = h * io.group + r - t * io.group;
     const long long row = (long long)(sp.t0 + t) * io.Hq + head;
     const int pos = sp.len - sp.n + t;
@@ -601,28 +906,44 @@ __global__ __launch_bounds__(256) void ca_paged_combine_kernel(PagedAttnIO io) {
     if (ns > io.splits) ns = io.splits;
     float m = kNegBig, z = 0.f;
     f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int s = sub; s < ns; s += kLanes) {
-      const long long at = s * nrows + row;
-      const float pm = io.part_ml[2 * at], pz = io.part_ml[2 * at + 1];
-      const f32x4 po = d < c.D ? ld4(io.part_o + at * c.D + d) : f32x4{0.f, 0.f, 0.f, 0.f};
+    auto add = [&](float pm, float pz, f32x4 po) {
       const float mn = fmaxf(m, pm);
       const float a = fast_exp2(m - mn), e = fast_exp2(pm - mn);
       o = o * a + po * e;
       z = z * a + pz * e;
       m = mn;
+    };
+#pragma unroll 4
+    for (int s = sub; s < ns; s += kLanes * WPR) {
+      const long long at = s * nrows + row;
+      const float2 ml = *reinterpret_cast<const float2*>(io.part_ml + 2 * at);
+      add(ml.x, ml.y, d < c.D ? ld4(io.part_o + at * c.D + d) : f32x4{0.f, 0.f, 0.f, 0.f});
     }
 #pragma unroll
     for (int x = kQuads; x < 64; x <<= 1) {
       const float pm = __shfl_xor(m, x), pz = __shfl_xor(z, x);
-      const float mn = fmaxf(m, pm);
-      const float a = fast_exp2(m - mn), e = fast_exp2(pm - mn);
+      f32x4 po;
 #pragma unroll
-      for (int y = 0; y < 4; ++y) o[y] = o[y] * a + __shfl_xor(o[y], x) * e;
-      z = z * a + pz * e;
-      m = mn;
+      for (int y = 0; y < 4; ++y) po[y] = __shfl_xor(o[y], x);
+      add(pm, pz, po);
+    }
+    if constexpr (WPR > 1) {
+      if (lane < kQuads) st4(&join[wave][d], o);
+      if (lane == 0) {
+        join[wave][DT] = m;
+        join[wave][DT + 1] = z;
+      }
+      __syncthreads();
+      m = kNegBig;
+      z = 0.f;
+      o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) add(join[w][DT], join[w][DT + 1], ld4(&join[w][d]));
+      __syncthreads();
+      if (wave > 0) continue;
     }
     const float inv = z == 0.f ? 0.f : 1.0f / z;
-    if (sub == 0 && d < c.D)
+    if (lane < kQuads && d < c.D)
       st4(static_cast<E*>(io.out) + (long long)(sp.t0 + t) * io.o_ts + (long long)head * io.o_hs + d, o * inv);
     if (io.stats && lane == 0) {
       io.stats[2 * row] = m;
@@ -699,20 +1020,25 @@ __global__ __launch_bounds__(256) void ca_paged_sums_kernel(PagedAttnIO io) {
 }
 
 template <class E, int DT>
-hipError_t run_attention(const PagedAttnIO& io, int wave_rows, hipStream_t s) {
-  const long long blocks = (long long)io.c.batch * io.c.heads * io.splits * io.row_tiles;
-  if (wave_rows == 1)
-    hipLaunchKernelGGL((ca_paged_attention_kernel<E, DT, 1>), dim3((unsigned)blocks), dim3(256), 0, s, io);
+hipError_t run_attention(const PagedAttnIO& io, hipStream_t s) {
+  const dim3 grid((unsigned)((long long)io.c.batch * io.c.heads * io.splits * io.row_tiles)), block(256);
+  if (io.tile_group == 0)
+    hipLaunchKernelGGL((ca_paged_attention_kernel<E, DT>), grid, block, 0, s, io);
+  else if (io.c.div.size % 32 == 0 && io.c.row_stride < 1 << 25)  // offsets within a tile in 32 bits
+    hipLaunchKernelGGL((ca_paged_few_kernel<E, DT, true>), grid, block, 0, s, io);
   else
-    hipLaunchKernelGGL((ca_paged_attention_kernel<E, DT, 4>), dim3((unsigned)blocks), dim3(256), 0, s, io);
+    hipLaunchKernelGGL((ca_paged_few_kernel<E, DT, false>), grid, block, 0, s, io);
   return hipGetLastError();
 }
 template <class E, int DT>
 hipError_t run_combine(const PagedAttnIO& io, hipStream_t s) {
   const long long slices = (long long)io.c.batch * io.c.heads;
-  const long long per = ((long long)io.tokens * io.group / io.c.batch + 3) / 4;
-  const long long parts = per < 1 ? 1 : per > 256 ? 256 : per;
-  hipLaunchKernelGGL((ca_paged_combine_kernel<E, DT>), dim3((unsigned)(slices * parts)), dim3(256), 0, s, io);
+  const bool wide = io.splits > 8 * (256 / DT);  // more than two rounds of one wave
+  const long long rows = (long long)io.tokens * io.group / io.c.batch;
+  const long long per = wide ? rows : (rows + 3) / 4;
+  const dim3 grid((unsigned)(slices * (per < 1 ? 1 : per > 256 ? 256 : per))), block(256);
+  if (wide) hipLaunchKernelGGL((ca_paged_combine_kernel<E, DT, 4>), grid, block, 0, s, io);
+  else hipLaunchKernelGGL((ca_paged_combine_kernel<E, DT, 1>), grid, block, 0, s, io);
   return hipGetLastError();
 }
 template <class E, int DT>
@@ -738,9 +1064,9 @@ template <class F> hipError_t by_type(int dtype, int D, F f) {
 
 }  // namespace
 
-hipError_t launch_paged_attention(const PagedAttnIO& io, int dtype, int wave_rows, hipStream_t s) {
+hipError_t launch_paged_attention(const PagedAttnIO& io, int dtype, hipStream_t s) {
   return by_type(dtype, io.c.D, [&](auto width, auto* e) {
-    return run_attention<std::remove_pointer_t<decltype(e)>, decltype(width)::value>(io, wave_rows, s);
+    return run_attention<std::remove_pointer_t<decltype(e)>, decltype(width)::value>(io, s);
   });
 }
 hipError_t launch_paged_combine(const PagedAttnIO& io, int dtype, hipStream_t s) {

@@ -72,11 +72,14 @@ ca::PagedCache kernel_cache(const ca_paged_cache& c) {
 // How the attention's grid is cut.  max_new and max_length only size it: the
 // kernels read what is there from the device and walk all of it.
 struct AttnPlan {
-  int wave_rows, row_tiles, splits, split_keys;
+  int row_tiles, splits, split_keys, row_log, tile_group;
 };
-constexpr int kOwnedKeys = 30;    // keys of a tile (ca_paged.hip)
-constexpr int kTargetGroups = 1024;  // four work groups on each of 256 CUs
-constexpr int kLeastTiles = 8;    // tiles of a split
+constexpr int kFewRows = 16;         // rows per key head that share a wave's columns
+constexpr int kTargetGroups = 2048;  // eight work groups for each of 256 CUs
+// with so many row tiles the device is full and partial sums cost more than
+// they even out: [2,2048] fp32 prompts in two splits 355 against 310 us
+constexpr int kEnoughGroups = 1024;
+constexpr int kLeastTiles = 8;       // tiles of a split (many rows)
 constexpr int kMostSplits = 128;
 
 size_t partial_bytes(int splits, int tokens, int heads, int D) {
@@ -84,19 +87,38 @@ size_t partial_bytes(int splits, int tokens, int heads, int D) {
 }
 AttnPlan attn_plan(int batch, int kv_heads, int heads, int D, int tokens, int max_new, int max_length) {
   const long long rows = (long long)std::max(1, std::min(max_new, tokens)) * (heads / kv_heads);
-  AttnPlan p;
-  p.wave_rows = rows <= 16 ? 1 : 4;
-  const long long tiles = (rows + 16 * p.wave_rows - 1) / (16 * p.wave_rows);
   const long long slices = (long long)batch * kv_heads;
-  const int key_tiles = std::max(1, (max_length + kOwnedKeys - 1) / kOwnedKeys);
-  long long splits = std::max<long long>(1, kTargetGroups / std::max<long long>(1, slices * tiles));
-  splits = std::min<long long>(splits, std::max(1, key_tiles / kLeastTiles));
+  AttnPlan p;
+  int unit, least;  // keys that a split is a multiple of, and its least number of these
+  long long tiles;  // of rows
+  if (rows <= kFewRows) {
+    p.row_log = 0;
+    while ((1 << p.row_log) < rows) ++p.row_log;
+    tiles = 1;
+    // tiles of keys that share a wave: as many as leave the device two waves on
+    // each SIMD
+    p.tile_group = kFewRows >> p.row_log;
+    const long long key_tiles = std::max(1, (max_length + 31) / 32);
+    while (p.tile_group > 1 && slices * ((key_tiles + p.tile_group - 1) / p.tile_group) < kTargetGroups)
+      p.tile_group >>= 1;
+    unit = 32 * p.tile_group;
+    least = 4;  // one for each wave of a work group
+  } else {
+    p.row_log = p.tile_group = 0;
+    tiles = (rows + 63) / 64;
+    unit = 30;
+    least = kLeastTiles;
+  }
+  const int units = std::max(1, (max_length + unit - 1) / unit);
+  long long splits = std::max<long long>(1, kTargetGroups / (slices * tiles));
+  if (!p.tile_group && slices * tiles >= kEnoughGroups) splits = 1;
+  splits = std::min<long long>(splits, std::max(1, units / least));
   splits = std::min<long long>(splits, kMostSplits);
   const size_t cap = ca_workspace_cap();
   while (splits > 1 && cap && partial_bytes((int)splits, tokens, heads, D) > cap) --splits;
-  const int per = (key_tiles + (int)splits - 1) / (int)splits;
-  p.splits = (key_tiles + per - 1) / per;
-  p.split_keys = per * kOwnedKeys;
+  const int per = (units + (int)splits - 1) / (int)splits;
+  p.splits = (units + per - 1) / per;
+  p.split_keys = per * unit;
   // at most 2^31 - 1 work groups
   p.row_tiles = (int)std::max<long long>(1, std::min<long long>(tiles, ((1ll << 31) - 1) / (slices * p.splits)));
   return p;
@@ -175,8 +197,10 @@ int ca_paged_attention(const ca_paged_cache* cache, const void* q, long long q_t
   io.splits = p.splits;
   io.split_keys = p.split_keys;
   io.row_tiles = p.row_tiles;
+  io.row_log = p.row_log;
+  io.tile_group = p.tile_group;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  hipError_t err = ca::launch_paged_attention(io, cache->dtype, p.wave_rows, s);
+  hipError_t err = ca::launch_paged_attention(io, cache->dtype, s);
   if (err == hipSuccess && p.splits > 1) err = ca::launch_paged_combine(io, cache->dtype, s);
   if (err == hipSuccess && sums) err = ca::launch_paged_sums(io, cache->dtype, max_length, s);
   if (err != hipSuccess) return set_error(CA_ERR_HIP, "%s launch: %s", op, hipGetErrorString(err));

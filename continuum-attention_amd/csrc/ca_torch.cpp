@@ -423,6 +423,394 @@ py::object weights(py::handle so) {
   return py::reinterpret_steal<py::object>(THPVariable_Wrap(w));
 }
 
+// ---- generation ----------------------------------------------------------------------
+//
+// The Python entry points of rotary.py, paged.py and int4.py call these first.
+// A call these refuse (None) is checked, and carried out or reported, there.
+
+// On a GPU, strided, not negated, no forward-mode dual.
+bool readable(const Tensor& t) {
+  return t.is_cuda() && t.layout() == at::kStrided && !t.is_neg() && !t._fw_grad(/*level=*/0).defined();
+}
+// 32-bit integers [..] on `device`, contiguous.
+bool counts(const Tensor& t, c10::Device device) {
+  return t.scalar_type() == at::kInt && t.device() == device && t.is_contiguous();
+}
+// Rows of a token tensor: [tokens, heads, D] of any strides with contiguous
+// rows, or more leading dims, contiguous.
+struct HeadRows {
+  int64_t tokens, heads, D, ts, hs;
+  bool ok;
+};
+HeadRows head_rows(const Tensor& t) {
+  HeadRows r{0, 0, 0, 0, 0, false};
+  if (t.dim() < 3) return r;
+  r.D = t.size(-1);
+  r.heads = t.size(-2);
+  if (r.D <= 0 || r.heads <= 0 || t.numel() == 0) return r;
+  r.tokens = t.numel() / (r.D * r.heads);
+  if (r.tokens > (1 << 30) || r.heads > (1 << 20)) return r;
+  if (t.dim() == 3) {
+    r.ok = t.stride(2) == 1;
+    r.ts = t.stride(0);
+    r.hs = t.stride(1);
+  } else {
+    r.ok = t.is_contiguous();
+    r.hs = r.D;
+    r.ts = r.heads * r.D;
+  }
+  return r;
+}
+
+struct RotaryPlan {
+  double magnitude;
+  int64_t half, rotary_dim, inverse;
+};
+// q (and k, if defined) turned; the arguments have been checked
+variable_list turn(const Tensor& q, const Tensor& k, const Tensor& positions, const Tensor& turns,
+                   const RotaryPlan& p) {
+  const c10::DeviceGuard guard(q.device());
+  ca_rotary r{};
+  auto rows = [](const Tensor& x, Tensor& held, int64_t& ts, int64_t& hs) {
+    held = x.detach().resolve_neg();
+    HeadRows h = head_rows(held);
+    if (!h.ok) {
+      held = held.contiguous();
+      h = head_rows(held);
+    }
+    ts = h.ts;
+    hs = h.hs;
+    return h;
+  };
+  Tensor qh, kh;
+  int64_t ts, hs;
+  const HeadRows a = rows(q, qh, ts, hs);
+  Tensor qo = empty(q.sizes(), q, q.scalar_type()), ko;
+  r.q = qh.const_data_ptr();
+  r.q_out = qo.data_ptr();
+  r.q_token_stride = ts;
+  r.q_head_stride = hs;
+  r.q_out_token_stride = a.heads * a.D;
+  r.q_out_head_stride = a.D;
+  if (k.defined()) {
+    const HeadRows b = rows(k, kh, ts, hs);
+    ko = empty(k.sizes(), k, k.scalar_type());
+    r.k = kh.const_data_ptr();
+    r.k_out = ko.data_ptr();
+    r.k_token_stride = ts;
+    r.k_head_stride = hs;
+    r.k_out_token_stride = b.heads * b.D;
+    r.k_out_head_stride = b.D;
+    r.k_heads = (int)b.heads;
+  }
+  r.positions = positions.const_data_ptr();
+  r.positions64 = positions.scalar_type() == at::kLong;
+  r.turns = turns.const_data_ptr<double>();
+  r.magnitude = (float)p.magnitude;
+  r.half = (int)p.half;
+  r.inverse = (int)p.inverse;
+  r.dtype = dtype_code(q.scalar_type());
+  r.tokens = (int)a.tokens;
+  r.q_heads = (int)a.heads;
+  r.head_dim = (int)a.D;
+  r.rotary_dim = (int)p.rotary_dim;
+  check(ca_rotary_embedding(&r, stream_of(q)));
+  return {qo, ko};
+}
+
+struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const std::optional<Tensor>& k_or_none,
+                               const Tensor& positions, const Tensor& turns, double magnitude, int64_t half, int64_t rotary_dim,
+                               int64_t inverse) {
+    ctx->save_for_backward({positions, turns});
+    ctx->saved_data["magnitude"] = magnitude;
+    ctx->saved_data["plan"] = std::vector<int64_t>{half, rotary_dim, inverse};
+    ctx->set_materialize_grads(false);
+    const Tensor k = k_or_none ? *k_or_none : Tensor();
+    variable_list y = turn(q, k, positions, turns, RotaryPlan{magnitude, half, rotary_dim, inverse});
+    if (!k.defined()) y.pop_back();
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    const std::vector<int64_t> p = ctx->saved_data["plan"].toIntVector();
+    const double magnitude = ctx->saved_data["magnitude"].toDouble();
+    variable_list out(8);
+    std::vector<int> which;
+    for (int i = 0; i < (int)grads.size(); ++i)
+      if (grads[i].defined()) which.push_back(i);
+    if (which.empty()) return out;
+    const Tensor a = grads[which[0]];
+    std::optional<Tensor> b;
+    if (which.size() > 1) b = grads[which[1]];
+    on_one_gpu("rotary_embedding", {&a, &saved[0], &saved[1]});
+    // the transpose is the rotation back; under create_graph it is recorded like it
+    const variable_list y = apply(a, b, saved[0], saved[1], magnitude, p[0], p[1], 1 - p[2]);
+    for (int i = 0; i < (int)which.size(); ++i) out[which[i]] = y[i];
+    return out;
+  }
+};
+
+py::object rotary(py::handle qo, py::handle ko, py::handle po, py::handle to, double magnitude, bool half,
+                  int64_t rotary_dim) {
+  if (!plain(qo.ptr()) || !plain(po.ptr()) || !plain(to.ptr()) || !(ko.is_none() || plain(ko.ptr())))
+    return py::none();
+  const Tensor q = THPVariable_Unpack(qo.ptr()), pos = THPVariable_Unpack(po.ptr()), turns = THPVariable_Unpack(to.ptr());
+  const Tensor k = ko.is_none() ? Tensor() : THPVariable_Unpack(ko.ptr());
+  if (!plain_context() || !readable(q) || (k.defined() && !readable(k))) return py::none();
+  const HeadRows a = head_rows(q);
+  if (!a.ok || dtype_code(q.scalar_type()) < 0 || turns.scalar_type() != at::kDouble || !turns.is_contiguous() ||
+      turns.numel() * 2 != rotary_dim || turns.device() != q.device() || pos.device() != q.device() ||
+      (pos.scalar_type() != at::kLong && pos.scalar_type() != at::kInt) || !pos.is_contiguous() ||
+      pos.numel() != a.tokens || pos.dim() != q.dim() - 2)
+    return py::none();
+  for (int64_t i = 0; i < pos.dim(); ++i)
+    if (pos.size(i) != q.size(i)) return py::none();
+  if (k.defined()) {
+    const HeadRows b = head_rows(k);
+    if (!b.ok || b.D != a.D || k.scalar_type() != q.scalar_type() || k.device() != q.device() || k.dim() != q.dim())
+      return py::none();
+    for (int64_t i = 0; i < pos.dim(); ++i)
+      if (k.size(i) != q.size(i)) return py::none();
+  }
+  variable_list y;
+  {
+    py::gil_scoped_release release;
+    if (grads_needed({&q}) || (k.defined() && grads_needed({&k})))
+      y = RotaryFunction::apply(q, k.defined() ? std::optional<Tensor>(k) : std::nullopt, pos, turns, magnitude, (int64_t)half, rotary_dim, (int64_t)0);
+    else
+      y = turn(q, k, pos, turns, RotaryPlan{magnitude, half, rotary_dim, 0});
+  }
+  py::object yk = py::none();
+  if (k.defined()) yk = py::reinterpret_steal<py::object>(THPVariable_Wrap(y[1]));
+  return py::make_tuple(py::reinterpret_steal<py::object>(THPVariable_Wrap(y[0])), yk);
+}
+
+// The C description of a cache; false: Python checks it
+bool describe(const Tensor& k, const Tensor& v, const Tensor& table, const Tensor& lengths, const Tensor* starts,
+              int64_t tokens, ca_paged_cache& c) {
+  if (!readable(k) || !readable(v) || k.dim() != 4 || v.sizes() != k.sizes() || v.strides() != k.strides() ||
+      v.scalar_type() != k.scalar_type() || dtype_code(k.scalar_type()) < 0 || v.device() != k.device() ||
+      k.numel() == 0 || k.stride(3) != 1)
+    return false;
+  for (int i = 0; i < 4; ++i)
+    if (k.size(i) > (1 << 30)) return false;
+  const c10::Device device = k.device();
+  if (!counts(table, device) || table.dim() != 2 || table.numel() == 0 || !counts(lengths, device) ||
+      lengths.dim() != 1 || lengths.size(0) != table.size(0) || table.size(0) > (1 << 24) || table.size(1) > (1 << 30))
+    return false;
+  if (starts && (!counts(*starts, device) || starts->dim() != 1 || starts->size(0) != table.size(0) + 1)) return false;
+  c = ca_paged_cache{};
+  c.k = const_cast<void*>(k.const_data_ptr());
+  c.v = const_cast<void*>(v.const_data_ptr());
+  c.table = table.const_data_ptr<int>();
+  c.lengths = lengths.const_data_ptr<int>();
+  c.starts = starts ? starts->const_data_ptr<int>() : nullptr;
+  c.page_stride = k.stride(0);
+  c.head_stride = k.stride(1);
+  c.row_stride = k.stride(2);
+  c.table_stride = table.size(1);
+  c.dtype = dtype_code(k.scalar_type());
+  c.heads = (int)k.size(1);
+  c.head_dim = (int)k.size(3);
+  c.page_size = (int)k.size(2);
+  c.num_pages = (int)k.size(0);
+  c.pages_per_seq = (int)table.size(1);
+  c.batch = (int)table.size(0);
+  c.tokens = (int)tokens;
+  return true;
+}
+bool shares_memory(const Tensor& a, const Tensor& b) {
+  return a.storage().unsafeGetStorageImpl() == b.storage().unsafeGetStorageImpl() || a.const_data_ptr() == b.const_data_ptr() ||
+         a.storage().data() == b.storage().data();
+}
+bool good_out(const Tensor& out, const Tensor& q) {
+  return readable(out) && out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type() &&
+         out.device() == q.device() && out.stride(2) == 1 && !shares_memory(out, q) && !grads_needed({&out});
+}
+
+py::object append(py::handle qo, py::handle ko, py::handle vo, py::handle po, py::handle to, double magnitude,
+                  bool half, int64_t rotary_dim, py::handle kpo, py::handle vpo, py::handle table_o,
+                  py::handle lengths_o, py::handle starts_o, py::handle oo) {
+  for (const py::handle& o : {qo, ko, vo, po, to, kpo, vpo, table_o, lengths_o, starts_o})
+    if (!plain(o.ptr())) return py::none();
+  if (!oo.is_none() && !plain(oo.ptr())) return py::none();
+  const Tensor q = THPVariable_Unpack(qo.ptr()), k = THPVariable_Unpack(ko.ptr()), v = THPVariable_Unpack(vo.ptr()),
+               pos = THPVariable_Unpack(po.ptr()), turns = THPVariable_Unpack(to.ptr()), kp = THPVariable_Unpack(kpo.ptr()),
+               vp = THPVariable_Unpack(vpo.ptr()), table = THPVariable_Unpack(table_o.ptr()),
+               lengths = THPVariable_Unpack(lengths_o.ptr()), starts = THPVariable_Unpack(starts_o.ptr());
+  if (!plain_context() || !readable(q) || !readable(k) || !readable(v) || q.dim() != 3 || k.dim() != 3 ||
+      k.sizes() != v.sizes() || grads_needed({&q, &k, &v, &kp, &vp}))
+    return py::none();
+  const HeadRows a = head_rows(q), b = head_rows(k), w = head_rows(v);
+  if (!a.ok || !b.ok || !w.ok || a.tokens != b.tokens || a.D != b.D || k.scalar_type() != q.scalar_type() ||
+      v.scalar_type() != q.scalar_type() || kp.scalar_type() != q.scalar_type() || kp.device() != q.device() ||
+      k.device() != q.device() || v.device() != q.device())
+    return py::none();
+  if (turns.scalar_type() != at::kDouble || !turns.is_contiguous() || turns.numel() * 2 != rotary_dim ||
+      turns.device() != q.device() || pos.device() != q.device() || pos.dim() != 1 || pos.numel() != a.tokens ||
+      (pos.scalar_type() != at::kLong && pos.scalar_type() != at::kInt) || !pos.is_contiguous())
+    return py::none();
+  ca_paged_cache c;
+  if (!describe(kp, vp, table, lengths, &starts, a.tokens, c) || c.heads != b.heads || c.head_dim != b.D)
+    return py::none();
+  Tensor out;
+  if (!oo.is_none()) {
+    out = THPVariable_Unpack(oo.ptr());
+    if (!good_out(out, q)) return py::none();
+  }
+  {
+    py::gil_scoped_release release;
+    const c10::DeviceGuard guard(q.device());
+    if (!out.defined()) out = empty(q.sizes(), q, q.scalar_type());
+    ca_rotary r{};
+    r.q = q.const_data_ptr();
+    r.k = k.const_data_ptr();
+    r.q_out = out.data_ptr();
+    r.positions = pos.const_data_ptr();
+    r.turns = turns.const_data_ptr<double>();
+    r.q_token_stride = a.ts;
+    r.q_head_stride = a.hs;
+    r.k_token_stride = b.ts;
+    r.k_head_stride = b.hs;
+    r.q_out_token_stride = out.stride(0);
+    r.q_out_head_stride = out.stride(1);
+    r.magnitude = (float)magnitude;
+    r.positions64 = pos.scalar_type() == at::kLong;
+    r.half = half;
+    r.dtype = c.dtype;
+    r.tokens = (int)a.tokens;
+    r.q_heads = (int)a.heads;
+    r.k_heads = (int)b.heads;
+    r.head_dim = (int)a.D;
+    r.rotary_dim = (int)rotary_dim;
+    check(ca_rotary_append(&r, v.const_data_ptr(), w.ts, w.hs, &c, stream_of(q)));
+  }
+  return py::reinterpret_steal<py::object>(THPVariable_Wrap(out));
+}
+
+// max_new, max_length: -1 for the defaults
+py::object attend(py::handle qo, py::handle kpo, py::handle vpo, py::handle table_o, py::handle lengths_o,
+                  py::handle starts_o, py::handle go, int64_t max_new, int64_t max_length, py::handle so,
+                  py::handle oo) {
+  for (const py::handle& o : {qo, kpo, vpo, table_o, lengths_o, starts_o, go})
+    if (!plain(o.ptr())) return py::none();
+  for (const py::handle& o : {so, oo})
+    if (!o.is_none() && !plain(o.ptr())) return py::none();
+  const Tensor q = THPVariable_Unpack(qo.ptr()), kp = THPVariable_Unpack(kpo.ptr()), vp = THPVariable_Unpack(vpo.ptr()),
+               table = THPVariable_Unpack(table_o.ptr()), lengths = THPVariable_Unpack(lengths_o.ptr()),
+               starts = THPVariable_Unpack(starts_o.ptr()), gain = THPVariable_Unpack(go.ptr());
+  if (!plain_context() || !readable(q) || q.dim() != 3 || !usable(gain) || gain.scalar_type() != at::kFloat ||
+      grads_needed({&q, &kp, &vp, &gain}) || max_new < -1 || max_length < -1)
+    return py::none();
+  const HeadRows a = head_rows(q);
+  const int64_t esize = q.element_size();
+  ca_paged_cache c;
+  if (!a.ok || !describe(kp, vp, table, lengths, &starts, a.tokens, c) || kp.device() != q.device() ||
+      q.scalar_type() != kp.scalar_type() || c.head_dim != a.D || a.D % 8 || a.D > 128 || a.heads % c.heads ||
+      gain.numel() != a.heads || gain.device() != q.device() || !aligned(q) || a.ts * esize % 16 || a.hs * esize % 16)
+    return py::none();
+  const int64_t capacity = (int64_t)c.pages_per_seq * c.page_size;
+  if (capacity > (1 << 30)) return py::none();
+  if (max_new < 0) max_new = a.tokens;
+  if (max_length < 0 || max_length > capacity) max_length = capacity;
+  max_new = std::min(max_new, a.tokens);
+  Tensor sums, out;
+  if (!so.is_none()) {
+    sums = THPVariable_Unpack(so.ptr());
+    if (!readable(sums) || sums.dim() != 3 || sums.scalar_type() != at::kFloat || sums.size(0) != c.batch ||
+        sums.size(1) != c.heads || sums.numel() == 0 || sums.stride(2) != 1 || sums.device() != q.device() ||
+        sums.size(2) > (1 << 30) || grads_needed({&sums}))
+      return py::none();
+  }
+  if (!oo.is_none()) {
+    out = THPVariable_Unpack(oo.ptr());
+    if (!good_out(out, q) || !aligned(out) || out.stride(0) * esize % 16 || out.stride(1) * esize % 16) return py::none();
+  }
+  {
+    py::gil_scoped_release release;
+    const c10::DeviceGuard guard(q.device());
+    if (!out.defined()) out = empty(q.sizes(), q, q.scalar_type());
+    const size_t bytes = ca_paged_attention_workspace_bytes(c.batch, c.heads, (int)a.heads, c.head_dim, c.tokens,
+                                                            (int)max_new, (int)max_length, sums.defined());
+    Tensor ws;
+    if (bytes) ws = workspace(bytes, q);
+    check(ca_paged_attention(&c, q.const_data_ptr(), a.ts, a.hs, (int)a.heads, gain.const_data_ptr<float>(),
+                             out.data_ptr(), out.stride(0), out.stride(1),
+                             sums.defined() ? sums.data_ptr<float>() : nullptr, sums.defined() ? sums.stride(0) : 0,
+                             sums.defined() ? sums.stride(1) : 0, sums.defined() ? (int)sums.size(2) : 0, (int)max_new,
+                             (int)max_length, bytes ? ws.data_ptr() : nullptr, bytes, stream_of(q)));
+  }
+  return py::reinterpret_steal<py::object>(THPVariable_Wrap(out));
+}
+
+py::object evict(py::handle kpo, py::handle vpo, py::handle table_o, py::handle lengths_o, py::handle so,
+                 py::handle new_o, int64_t budget, int64_t sinks, int64_t recent) {
+  for (const py::handle& o : {kpo, vpo, table_o, lengths_o, so, new_o})
+    if (!plain(o.ptr())) return py::none();
+  const Tensor kp = THPVariable_Unpack(kpo.ptr()), vp = THPVariable_Unpack(vpo.ptr()), table = THPVariable_Unpack(table_o.ptr()),
+               lengths = THPVariable_Unpack(lengths_o.ptr()), sums = THPVariable_Unpack(so.ptr()),
+               to = THPVariable_Unpack(new_o.ptr());
+  ca_paged_cache c;
+  if (!plain_context() || grads_needed({&kp, &vp, &sums}) || !describe(kp, vp, table, lengths, nullptr, 0, c) ||
+      !readable(sums) || sums.dim() != 3 || sums.scalar_type() != at::kFloat || sums.size(0) != c.batch ||
+      sums.size(1) != c.heads || sums.numel() == 0 || sums.stride(2) != 1 || sums.device() != kp.device() ||
+      sums.size(2) > (1 << 30) || !counts(to, kp.device()) || to.dim() != 2 || to.size(0) != c.batch ||
+      budget <= 0 || budget > (1 << 30) || sinks < 0 || recent < 0 || sinks + recent > budget ||
+      to.size(1) * c.page_size < budget)
+    return py::none();
+  Tensor kept, lens, new_sums;
+  {
+    py::gil_scoped_release release;
+    const c10::DeviceGuard guard(kp.device());
+    kept = empty({c.batch, c.heads, budget}, kp, at::kInt);
+    new_sums = empty({c.batch, c.heads, budget}, kp, at::kFloat);
+    lens = empty({c.batch}, kp, at::kInt);
+    check(ca_evict(&c, sums.const_data_ptr<float>(), sums.stride(0), sums.stride(1), (int)sums.size(2), (int)budget,
+                   (int)sinks, (int)recent, to.const_data_ptr<int>(), to.size(1), kept.data_ptr<int>(),
+                   new_sums.data_ptr<float>(), lens.data_ptr<int>(), stream_of(kp)));
+  }
+  return py::make_tuple(py::reinterpret_steal<py::object>(THPVariable_Wrap(kept)),
+                        py::reinterpret_steal<py::object>(THPVariable_Wrap(lens)),
+                        py::reinterpret_steal<py::object>(THPVariable_Wrap(new_sums)));
+}
+
+// weight: an Int4Weight's tensors, checked when it was made
+py::object int4_product(py::handle xo, py::handle co, py::handle so, py::handle zo, int64_t K, int64_t group) {
+  for (const py::handle& o : {xo, co, so})
+    if (!plain(o.ptr())) return py::none();
+  if (!zo.is_none() && !plain(zo.ptr())) return py::none();
+  const Tensor x = THPVariable_Unpack(xo.ptr()), codes = THPVariable_Unpack(co.ptr()), scales = THPVariable_Unpack(so.ptr());
+  const Tensor zeros = zo.is_none() ? Tensor() : THPVariable_Unpack(zo.ptr());
+  if (!plain_context() || !readable(x) || x.dim() < 1 || x.numel() == 0 || x.size(-1) != K || grads_needed({&x}) ||
+      dtype_code(x.scalar_type()) < 0 || scales.scalar_type() != x.scalar_type() || codes.device() != x.device() ||
+      !usable(codes) || codes.dim() != 2 || codes.scalar_type() != at::kInt || codes.size(1) != (K + 127) / 128 * 16 ||
+      !scales.is_contiguous() || scales.device() != x.device() || group <= 0 ||
+      scales.numel() != (K + group - 1) / group * codes.size(0) ||
+      (zeros.defined() && (zeros.scalar_type() != x.scalar_type() || !zeros.is_contiguous() ||
+                           zeros.numel() != scales.numel() || zeros.device() != x.device())))
+    return py::none();
+  const int64_t M = x.numel() / K, N = codes.size(0);
+  int64_t rs = K;
+  if (x.dim() == 2 && x.stride(1) == 1 && (x.stride(0) >= K || M == 1))
+    rs = std::max(x.stride(0), K);
+  else if (!x.is_contiguous())
+    return py::none();
+  if (M > (1 << 19) || N > (1 << 30) || K > (1 << 30)) return py::none();
+  Tensor y;
+  {
+    py::gil_scoped_release release;
+    const c10::DeviceGuard guard(x.device());
+    std::vector<int64_t> shape = x.sizes().vec();
+    shape.back() = N;
+    y = empty(shape, x, x.scalar_type());
+    check(ca_int4_linear(x.const_data_ptr(), rs, reinterpret_cast<const unsigned*>(codes.const_data_ptr<int>()),
+                         scales.const_data_ptr(), zeros.defined() ? zeros.const_data_ptr() : nullptr, y.data_ptr(), N,
+                         dtype_code(x.scalar_type()), (int)M, (int)N, (int)K, (int)group, stream_of(x)));
+  }
+  return py::reinterpret_steal<py::object>(THPVariable_Wrap(y));
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -433,4 +821,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rmsnorm", &rmsnorm);
   m.def("add_rmsnorm", &add_rmsnorm);
   m.def("weights", &weights);
+  m.def("rotary", &rotary);
+  m.def("append", &append);
+  m.def("attend", &attend);
+  m.def("evict", &evict);
+  m.def("int4", &int4_product);
 }

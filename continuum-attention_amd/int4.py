@@ -105,6 +105,12 @@ def int4_linear(x, weight: Int4Weight):
     Made for the few rows of a decoding step (any number works; the codes are
     read once per 16 or 32 rows).  No backward pass.  A row of x that holds an
     infinity gives NaN."""
+    # the plain case runs in native code (csrc/ca_torch.cpp); what it does not take is checked here
+    if x.is_cuda and not torch.compiler.is_compiling():
+        y = _native.torch_ext().int4(x, weight.codes, weight.scales, weight.zeros, weight.in_features,
+                                     weight.group_size)
+        if y is not None:
+            return y
     if torch.is_grad_enabled() and x.requires_grad:
         raise RuntimeError("int4_linear has no backward pass; call it under torch.no_grad()")
     K, N = weight.in_features, weight.out_features

@@ -38,6 +38,10 @@ def _refuse_grad(name, *tensors):
         raise RuntimeError(f"{name} has no backward pass; call it under torch.no_grad()")
 
 
+def _on_gpu(t):
+    return isinstance(t, torch.Tensor) and t.is_cuda and not torch.compiler.is_compiling()
+
+
 def _int32(name, t, shape, device):
     _require(isinstance(t, torch.Tensor) and t.dtype == torch.int32, f"{name} must be a tensor of 32-bit integers")
     _require(t.dim() == len(shape) and all(s is None or s == n for s, n in zip(shape, t.shape)),
@@ -114,6 +118,12 @@ def rotary_append(q, k, v, positions, rotary, k_pages, v_pages, page_table, leng
     Slots without a page of the cache are not written.  ``out`` receives q;
     without it rows that belong to no sequence are undefined.  ``max_new`` is
     accepted for symmetry with paged_attention and not needed."""
+    # the plain case runs in native code (csrc/ca_torch.cpp); what it does not take is checked here
+    if _on_gpu(q) and q.shape[-1] == rotary.head_dim:
+        y = _native.torch_ext().append(q, k, v, positions, rotary.turns, rotary.magnitude, rotary.layout == "half",
+                                       rotary.rotary_dim, k_pages, v_pages, page_table, lengths, starts, out)
+        if y is not None:
+            return y
     _refuse_grad("rotary_append", q, k, v, k_pages, v_pages)
     q3, k3 = _rows("q", q, rotary), _rows("k", k, rotary, q)
     v3 = _rows("v", v, rotary, q)
@@ -190,6 +200,13 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, starts, log_gain, 
     A token that sees no slot gets zeros; one that reads a page number outside
     the cache gets NaN.  ``out`` receives the result; without it rows that belong
     to no sequence are undefined."""
+    if _on_gpu(q):  # as in rotary_append
+        y = _native.torch_ext().attend(q, k_pages, v_pages, page_table, lengths, starts, log_gain,
+                                       -1 if max_new is None else int(max_new),
+                                       -1 if max_length is None else int(max_length),
+                                       weight_sums, out)
+        if y is not None:
+            return y
     _refuse_grad("paged_attention", q, k_pages, v_pages, log_gain)
     _require(isinstance(q, torch.Tensor) and q.dim() == 3, "q must be [tokens, heads, head_dim]")
     N, H, D = q.shape
@@ -283,6 +300,11 @@ def evict(k_pages, v_pages, page_table, lengths, weight_sums, new_table, budget,
     left as they were.  Returns ``(kept, new_lengths, new_sums)``: the kept
     slots' former numbers ``[B, kv_heads, budget]`` int32 (-1 behind the last),
     the new lengths ``[B]`` int32 and the kept slots' sums (0 behind the last)."""
+    if _on_gpu(k_pages):  # as in rotary_append
+        y = _native.torch_ext().evict(k_pages, v_pages, page_table, lengths, weight_sums, new_table, int(budget),
+                                      int(sinks), int(recent))
+        if y is not None:
+            return y
     _refuse_grad("evict", k_pages, v_pages, weight_sums)
     c = _cache(k_pages, v_pages, page_table, lengths, None, 0)
     dev = k_pages.device

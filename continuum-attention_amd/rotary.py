@@ -207,6 +207,13 @@ def rotary_embedding(q, k, positions, rotary):
     leading shape, in any strides; positions: integers of the leading shape, or
     one that expands to it.  Differentiable in q and k.  On the GPU one kernel
     each way; the results are contiguous, in the inputs' dtype, rounded once."""
+    # the plain case (see csrc/ca_torch.cpp) runs _RotaryFn's native counterpart
+    if (isinstance(q, torch.Tensor) and q.is_cuda and q.dim() > 2 and q.shape[-1] == rotary.head_dim
+            and not torch.compiler.is_compiling()):
+        y = _native.torch_ext().rotary(q, k, positions, rotary.turns, rotary.magnitude, rotary.layout == "half",
+                                       rotary.rotary_dim)
+        if y is not None:
+            return y
     _rows("q", q, rotary)
     if k is not None:
         _rows("k", k, rotary, q)
