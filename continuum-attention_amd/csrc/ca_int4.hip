@@ -11,15 +11,19 @@
 // in fp32: the offset is about as large as the codes, so this costs two or three
 // bits of the 24.  fp32 x goes through the bf16 form in three exact bf16 limbs.
 //
-// Tiles.  A wave takes 16 rows n and 128 columns k at a time: lane (i, r) loads
-// 16 bytes, the 32 codes k = 32 r .. 32 r + 31 of row i, and gives eight of them to
-// each of four 16x16x32 instructions, whose k indexes then stand for
-// k = 32 r + 8 j + e; x is read with the same deal.  Groups smaller than 128
-// share an instruction, so x is zeroed outside one group at a time.  The waves
-// of a work group deal out the columns and add up at the end in a fixed order.
+// Tiles.  A wave takes 16 rows n and 128 columns k at a time, stored as the 1 KB that
+// it reads with one load: lane (i, r) gets the codes of row i, columns
+// 32 j + 8 r + e, j = 0..3, e = 0..7, eight for each of four 16x16x32 instructions, so
+// that one instruction covers 32 neighbouring columns and no group is split by
+// one.  (Row by row, a load touched 16 lines, and the address unit bounded it:
+// [16,8192] x [8192,8192] 26 us.)  x passes through shared memory for the same
+// reason: read as 256 bytes of a row by 16 lanes, handed over as operands.  Each
+// group's sums are scaled where they end.  The waves of a work group deal out the
+// columns and add up at the end in a fixed order.
 //
 // Codes of a word (eight columns): column 2 p in bits 4 p, column 2 p + 1 in bits
-// 16 + 4 p, so that a shift by 4 p lines up a pair in the two halves.
+// 16 + 4 p, so that a shift by 4 p lines up a pair in the two halves.  Rows of
+// codes, and of scales and zero points ([group][row]), are padded to 16.
 #include "ca_int4.h"
 
 namespace ca {
@@ -48,44 +52,33 @@ __device__ __forceinline__ f32x4 product(u32x4 a, u32x4 b, f32x4 c) {
                                                   0, 0, 0);
 }
 
-// x[m][k .. k + 7] as operand limbs, zeros past K and M.
+// 16 bytes of a row of x at p, `left` columns before its end, element by element.
+template <class E>
+__device__ __forceinline__ u32x4 load_part(const E* p, int left) {
+  constexpr int kVec = 16 / sizeof(E);
+  u32x4 r = {0, 0, 0, 0};
+#pragma unroll
+  for (int e = 0; e < kVec; ++e) {
+    if (e >= left) break;
+    if constexpr (kVec == 8) r[e >> 1] |= (unsigned)reinterpret_cast<const unsigned short*>(p)[e] << (16 * (e & 1));
+    else r[e] = reinterpret_cast<const unsigned*>(p)[e];
+  }
+  return r;
+}
+// Eight values as operand limbs (16-bit values are their own).
 template <class E, int XL>
-__device__ __forceinline__ void load_x(const Int4IO& io, int m, int k, u32x4 (&out)[XL]) {
-  const E* p = static_cast<const E*>(io.x) + (long long)m * io.x_rs + k;
+__device__ __forceinline__ void operand_x(const E* p, u32x4 (&out)[XL]) {
   if constexpr (XL == 1) {
-    if (m < io.M && io.x_aligned && k + 8 <= io.K) {
-      out[0] = *reinterpret_cast<const u32x4*>(p);
-      return;
-    }
-    u32x4 r = {0, 0, 0, 0};
-    if (m < io.M) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const unsigned v = k + e < io.K ? reinterpret_cast<const unsigned short*>(p)[e] : 0u;
-        r[e >> 1] |= v << (16 * (e & 1));
-      }
-    }
-    out[0] = r;
+    out[0] = *reinterpret_cast<const u32x4*>(p);
   } else {
-    float v[8];
-    const bool fast = m < io.M && io.x_aligned && k + 8 <= io.K;
-    if (fast) {
-      const f32x4 a = ld4(p), b = ld4(p + 4);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        v[e] = a[e];
-        v[4 + e] = b[e];
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = m < io.M && k + e < io.K ? p[e] : 0.f;
-    }
+    const f32x4 a = ld4(p), b = ld4(p + 4);
+    const float v[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      unsigned h, mm, l;
-      split_pair(v[2 * q], v[2 * q + 1], h, mm, l);
+      unsigned h, m, l;
+      split_pair(v[2 * q], v[2 * q + 1], h, m, l);
       out[0][q] = h;
-      out[1][q] = mm;
+      out[1][q] = m;
       out[2][q] = l;
     }
   }
@@ -99,103 +92,147 @@ template <class E, int NT, int MT, int SUB>
 __global__ __launch_bounds__(64 * kMostWaves) void ca_int4_kernel(Int4IO io) {
   constexpr bool kBf = !std::is_same<E, _Float16>::value;
   constexpr int XL = std::is_same<E, float>::value ? 3 : 1;
-  __shared__ float join[kMostWaves][NT * MT][16 * 17];
+  constexpr int kPer = 4 / SUB;  // instructions of a group
+  constexpr int kVec = 16 / sizeof(E), kPieces = 128 / kVec;  // 16-byte pieces of a row's 128 columns
+  constexpr int kLoads = 16 * MT * kPieces / 64;              // of x per lane and block
+  constexpr int kXRow = 128 + kVec;                           // staged row: 16 bytes of padding
+  constexpr int kXBytes = 16 * MT * kXRow * (int)sizeof(E), kJoinBytes = NT * MT * 16 * 17 * 4;
+  __shared__ __attribute__((aligned(16))) unsigned char lds[kMostWaves][kXBytes > kJoinBytes ? kXBytes : kJoinBytes];
   const int lane = threadIdx.x & 63, i = lane & 15, r = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), waves = blockDim.x >> 6;
   const int n0 = blockIdx.x * 16 * NT, m0 = blockIdx.y * 16 * MT;
   const u32x4 ones = kBf ? u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u}
                          : u32x4{0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
-  const int blocks = (io.K + 127) / 128;
+  const int blocks = (io.K + 127) / 128, rows = (io.N + 15) / 16 * 16;
   const int per = SUB == 1 ? io.group / 128 : 1;  // blocks of a group
+  const int groups = (io.K + io.group - 1) / io.group;
   f32x4 y[NT][MT];
 #pragma unroll
   for (int a = 0; a < NT; ++a)
 #pragma unroll
     for (int b = 0; b < MT; ++b) y[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // (a work group's last tiles may lie behind the padded rows: their loads
+  // take the first tile's place and nothing of them is written)
+  int n[NT];
   const unsigned* row[NT];
 #pragma unroll
   for (int a = 0; a < NT; ++a) {
-    const int n = n0 + 16 * a + i;
-    row[a] = io.codes + (long long)(n < io.N ? n : io.N - 1) * io.row_words + 4 * r;
+    n[a] = n0 + 16 * a < rows ? n0 + 16 * a : n0;
+    row[a] = io.codes + (long long)(n[a] / 16) * blocks * 256 + 4 * lane;
   }
-  const E* scales = static_cast<const E*>(io.scales);
-  const E* zeros = static_cast<const E*>(io.zeros);
-  // a wave takes two neighbouring blocks at a time: 128 bytes of each row
-  for (int pair = wave; 2 * pair < blocks; pair += waves) {
-    const int first = 2 * pair, count = first + 1 < blocks ? 2 : 1;
-    u32x4 w[2][NT];
+  const E* x_row[kLoads];  // this lane's pieces of x
 #pragma unroll
-    for (int q = 0; q < 2; ++q)
+  for (int q = 0; q < kLoads; ++q) {
+    const int m = m0 + (lane + 64 * q) / kPieces;
+    x_row[q] = m < io.M ? static_cast<const E*>(io.x) + (long long)m * io.x_rs + lane % kPieces * kVec : nullptr;
+  }
+  // What a block of 128 columns needs, loaded one block ahead.
+  struct Block {
+    u32x4 codes[NT], x[kLoads];
+    typename Raw4<E>::type scale[SUB][NT], zero[SUB][NT];
+  };
+  auto load = [&](int block, Block& o) {
 #pragma unroll
-      for (int a = 0; a < NT; ++a)
-        w[q][a] = q < count ? *reinterpret_cast<const u32x4*>(row[a] + 16 * (first + q)) : u32x4{0, 0, 0, 0};
+    for (int a = 0; a < NT; ++a) o.codes[a] = *reinterpret_cast<const u32x4*>(row[a] + 256 * (long long)block);
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      if (q >= count) break;
-      const int block = first + q;
-      f32x4 acc[SUB][NT][MT], sum[SUB][MT];
+    for (int s = 0; s < SUB; ++s) {
+      int g = SUB == 1 ? block / per : SUB * block + s;
+      if (SUB > 1 && g >= groups) g = groups - 1;  // columns past K: x is zero there
 #pragma unroll
-      for (int s = 0; s < SUB; ++s)
+      for (int a = 0; a < NT; ++a) {
+        const long long at = (long long)g * rows + n[a] + 4 * r;
+        o.scale[s][a] = ld_raw4(static_cast<const E*>(io.scales) + at);
+        if (io.zeros) o.zero[s][a] = ld_raw4(static_cast<const E*>(io.zeros) + at);
+      }
+    }
+    // rows past M are zero; whole aligned blocks are the rule
+    if (io.x_aligned && 128 * block + 128 <= io.K) {
 #pragma unroll
-        for (int b = 0; b < MT; ++b) {
-          sum[s][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int q = 0; q < kLoads; ++q)
+        o.x[q] = x_row[q] ? *reinterpret_cast<const u32x4*>(x_row[q] + 128 * block) : u32x4{0, 0, 0, 0};
+    } else {
 #pragma unroll
-          for (int a = 0; a < NT; ++a) acc[s][a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
-        }
+      for (int q = 0; q < kLoads; ++q)
+        o.x[q] = x_row[q] ? load_part<E>(x_row[q] + 128 * block, io.K - 128 * block - lane % kPieces * kVec)
+                          : u32x4{0, 0, 0, 0};
+    }
+  };
+  E* xs = reinterpret_cast<E*>(lds[wave]);
+  auto add = [&](const Block& o) {
+    wave_lds_sync();  // the block before has been read
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        u32x4 x[MT][XL];
+    for (int q = 0; q < kLoads; ++q) {
+      const int at = lane + 64 * q;
+      *reinterpret_cast<u32x4*>(xs + at / kPieces * kXRow + at % kPieces * kVec) = o.x[q];
+    }
+    wave_lds_sync();
 #pragma unroll
-        for (int b = 0; b < MT; ++b) load_x<E, XL>(io, m0 + 16 * b + i, 128 * block + 32 * r + 8 * j, x[b]);
+    for (int s = 0; s < SUB; ++s) {
+      f32x4 sum[MT], acc[NT][MT];
 #pragma unroll
-        for (int s = 0; s < SUB; ++s) {
-          const bool in = SUB == 1 || r / (4 / SUB) == s;
+      for (int b = 0; b < MT; ++b) {
+        sum[b] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int b = 0; b < MT; ++b)
-#pragma unroll
-            for (int l = XL - 1; l >= 0; --l) {
-              const u32x4 v = in ? x[b][l] : u32x4{0, 0, 0, 0};
-              sum[s][b] = product<kBf>(ones, v, sum[s][b]);
-#pragma unroll
-              for (int a = 0; a < NT; ++a) acc[s][a][b] = product<kBf>(operand<kBf>(w[q][a][j]), v, acc[s][a][b]);
-            }
-        }
+        for (int a = 0; a < NT; ++a) acc[a][b] = f32x4{0.f, 0.f, 0.f, 0.f};
       }
 #pragma unroll
-      for (int s = 0; s < SUB; ++s) {
-        const int k = 128 * block + 128 / SUB * s;
-        if (k >= io.K) break;
-        const int g = SUB == 1 ? block / per : SUB * block + s;
+      for (int j = kPer * s; j < kPer * s + kPer; ++j) {
+        u32x4 c[NT];
 #pragma unroll
-        for (int a = 0; a < NT; ++a) {
+        for (int a = 0; a < NT; ++a) c[a] = operand<kBf>(o.codes[a][j]);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int n = n0 + 16 * a + 4 * r + e;
-            const long long at = (long long)g * io.N + (n < io.N ? n : io.N - 1);
-            const float sc = ld1(scales + at);
-            const float off = 16.0f + (zeros ? ld1(zeros + at) : 8.0f);
+        for (int b = 0; b < MT; ++b) {
+          u32x4 x[XL];
+          operand_x<E, XL>(xs + (16 * b + i) * kXRow + 32 * j + 8 * r, x);
 #pragma unroll
-            for (int b = 0; b < MT; ++b) y[a][b][e] = fmaf(sc, fmaf(-off, sum[s][b][e], acc[s][a][b][e]), y[a][b][e]);
+          for (int l = XL - 1; l >= 0; --l) {
+            sum[b] = product<kBf>(ones, x[l], sum[b]);
+#pragma unroll
+            for (int a = 0; a < NT; ++a) acc[a][b] = product<kBf>(c[a], x[l], acc[a][b]);
           }
         }
       }
+#pragma unroll
+      for (int a = 0; a < NT; ++a) {
+        const f32x4 sc = raw_to_f32(o.scale[s][a], (const E*)nullptr);
+        const f32x4 off = io.zeros ? raw_to_f32(o.zero[s][a], (const E*)nullptr) + 16.0f : f32x4{24.f, 24.f, 24.f, 24.f};
+#pragma unroll
+        for (int b = 0; b < MT; ++b)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[a][b][e] = fmaf(sc[e], fmaf(-off[e], sum[b][e], acc[a][b][e]), y[a][b][e]);
+      }
     }
+  };
+  auto block_of = [&](int k) { return wave + waves * k; };
+  Block p, q;
+  int k = 0;
+  if (block_of(0) < blocks) load(block_of(0), p);
+  while (block_of(k) < blocks) {
+    const bool more = block_of(k + 1) < blocks;
+    if (more) load(block_of(k + 1), q);
+    add(p);
+    if (!more) break;
+    if (block_of(k + 2) < blocks) load(block_of(k + 2), p);
+    add(q);
+    k += 2;
   }
+  wave_lds_sync();
+  float* join = reinterpret_cast<float*>(lds[wave]);
 #pragma unroll
   for (int a = 0; a < NT; ++a)
 #pragma unroll
     for (int b = 0; b < MT; ++b)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) join[wave][a * MT + b][(4 * r + e) * 17 + i] = y[a][b][e];
+      for (int e = 0; e < 4; ++e) join[(a * MT + b) * 272 + (4 * r + e) * 17 + i] = y[a][b][e];
   __syncthreads();
   E* out = static_cast<E*>(io.y);
   for (int u = threadIdx.x; u < 256 * NT * MT; u += blockDim.x) {
-    const int n = u % 16, m = u / 16 % 16, tile = u / 256;
-    const int nn = n0 + 16 * (tile / MT) + n, mm = m0 + 16 * (tile % MT) + m;
-    if (nn >= io.N || mm >= io.M) continue;
+    const int nn = u % 16, m = u / 16 % 16, tile = u / 256;
+    const int nr = n0 + 16 * (tile / MT) + nn, mr = m0 + 16 * (tile % MT) + m;
+    if (nr >= io.N || mr >= io.M) continue;
     float v = 0.f;
-    for (int w = 0; w < waves; ++w) v += join[w][tile][n * 17 + m];
-    st1(out + (long long)mm * io.y_rs + nn, v);
+    for (int q = 0; q < waves; ++q) v += reinterpret_cast<const float*>(lds[q])[tile * 272 + nn * 17 + m];
+    st1(out + (long long)mr * io.y_rs + nr, v);
   }
 }
 
@@ -208,13 +245,19 @@ hipError_t run_sub(const Int4IO& io, dim3 grid, dim3 block, hipStream_t s) {
 }
 template <class E>
 hipError_t run_int4(const Int4IO& io, hipStream_t s) {
-  const int pairs = (io.K + 255) / 256;
-  const int waves = pairs < kMostWaves ? pairs : kMostWaves;
-  const dim3 block(64 * waves);
-  const int mt = io.M <= 16 ? 1 : 2;
-  const dim3 grid((io.N + 15) / 16, (io.M + 16 * mt - 1) / (16 * mt));
-  if (mt == 1) return run_sub<E, 1, 1>(io, grid, block, s);
-  return run_sub<E, 1, 2>(io, grid, block, s);
+  const int blocks = (io.K + 127) / 128;
+  const dim3 block(64 * (blocks < kMostWaves ? blocks : kMostWaves));
+  // fp32 rows take twice the shared memory: 16 at a time
+  const int mt = io.M <= 16 || sizeof(E) == 4 ? 1 : 2;
+  const unsigned my = (io.M + 16 * mt - 1) / (16 * mt);
+  const int tiles = (io.N + 15) / 16;
+  if constexpr (sizeof(E) == 2) {
+    if (mt == 2) return run_sub<E, 1, 2>(io, dim3(tiles, my), block, s);
+    // two tiles share x where that still leaves a work group for each of 256 CUs
+    // ([16,8192] x [8192,8192] 16.4 -> 15.5 us; [1,1024] x [4096,1024] 3.6 -> 4.2)
+    if (tiles >= 512) return run_sub<E, 2, 1>(io, dim3((tiles + 1) / 2, my), block, s);
+  }
+  return run_sub<E, 1, 1>(io, dim3(tiles, my), block, s);
 }
 
 }  // namespace

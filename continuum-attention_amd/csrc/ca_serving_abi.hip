@@ -345,7 +345,7 @@ int ca_int4_linear(const void* x, long long x_stride, const unsigned* codes, con
   if (x_stride < K || y_stride < N) return set_error(CA_ERR_INVALID, "%s: row strides below the rows' lengths", op);
   if (M == 0) return CA_OK;
   if (!x || !codes || !scales || !y) return set_error(CA_ERR_INVALID, "%s: null pointer", op);
-  if (!aligned(codes, 16) || !aligned(x, e) || !aligned(scales, e) || !aligned(zeros, e) || !aligned(y, e))
+  if (!aligned(codes, 16) || !aligned(x, e) || !aligned(scales, 16) || !aligned(zeros, 16) || !aligned(y, e))
     return set_error(CA_ERR_INVALID, "%s: misaligned pointer", op);
   ca::Int4IO io;
   io.x = x;
@@ -359,7 +359,6 @@ int ca_int4_linear(const void* x, long long x_stride, const unsigned* codes, con
   io.N = N;
   io.K = K;
   io.group = group;
-  io.row_words = (K + 127) / 128 * 16;
   io.x_aligned = aligned(x, 16) && x_stride * e % 16 == 0;
   hipError_t err = ca::launch_int4(io, dtype, reinterpret_cast<hipStream_t>(stream));
   if (err != hipSuccess) return set_error(CA_ERR_HIP, "%s launch: %s", op, hipGetErrorString(err));

@@ -776,7 +776,7 @@ py::object evict(py::handle kpo, py::handle vpo, py::handle table_o, py::handle 
 }
 
 // weight: an Int4Weight's tensors, checked when it was made
-py::object int4_product(py::handle xo, py::handle co, py::handle so, py::handle zo, int64_t K, int64_t group) {
+py::object int4_product(py::handle xo, py::handle co, py::handle so, py::handle zo, int64_t N, int64_t K, int64_t group) {
   for (const py::handle& o : {xo, co, so})
     if (!plain(o.ptr())) return py::none();
   if (!zo.is_none() && !plain(zo.ptr())) return py::none();
@@ -784,13 +784,13 @@ py::object int4_product(py::handle xo, py::handle co, py::handle so, py::handle 
   const Tensor zeros = zo.is_none() ? Tensor() : THPVariable_Unpack(zo.ptr());
   if (!plain_context() || !readable(x) || x.dim() < 1 || x.numel() == 0 || x.size(-1) != K || grads_needed({&x}) ||
       dtype_code(x.scalar_type()) < 0 || scales.scalar_type() != x.scalar_type() || codes.device() != x.device() ||
-      !usable(codes) || codes.dim() != 2 || codes.scalar_type() != at::kInt || codes.size(1) != (K + 127) / 128 * 16 ||
-      !scales.is_contiguous() || scales.device() != x.device() || group <= 0 ||
-      scales.numel() != (K + group - 1) / group * codes.size(0) ||
-      (zeros.defined() && (zeros.scalar_type() != x.scalar_type() || !zeros.is_contiguous() ||
+      !usable(codes) || codes.scalar_type() != at::kInt || N <= 0 ||
+      codes.numel() != (N + 15) / 16 * ((K + 127) / 128) * 256 || !usable(scales) || scales.device() != x.device() || group <= 0 ||
+      scales.numel() != (K + group - 1) / group * ((N + 15) / 16 * 16) ||
+      (zeros.defined() && (zeros.scalar_type() != x.scalar_type() || !usable(zeros) ||
                            zeros.numel() != scales.numel() || zeros.device() != x.device())))
     return py::none();
-  const int64_t M = x.numel() / K, N = codes.size(0);
+  const int64_t M = x.numel() / K;
   int64_t rs = K;
   if (x.dim() == 2 && x.stride(1) == 1 && (x.stride(0) >= K || M == 1))
     rs = std::max(x.stride(0), K);

@@ -18,31 +18,40 @@ def _check_group(group_size):
         raise ValueError(f"groups of {group_size} columns: 32, 64 or a multiple of 128")
 
 
+def _aligned(t):
+    t = t.detach().resolve_neg().contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+# bits of a word's eight columns
+_BITS = (0, 16, 4, 20, 8, 24, 12, 28)
+
+
 class Int4Weight:
     """An ``[out, in]`` matrix of 4-bit codes as the kernel reads them.
 
-    ``codes`` int32 ``[out, ceil(in / 128) * 16]`` (word w holds columns
-    8w .. 8w + 7: column 8w + 2p in bits 4p, column 8w + 2p + 1 in bits 16 + 4p),
-    ``scales`` and ``zeros`` (or None: 8) ``[ceil(in / group), out]`` in the
-    activations' dtype."""
+    With the rows rounded up to a multiple of 16, ``codes`` is int32 ``[rows / 16,
+    ceil(in / 128), 64, 4]``, tiles of 16 rows by 128 columns: word (16r + i, j) holds
+    row i, columns c = 32j + 8r .. c + 7, column c + 2p in bits 4p and column c + 2p + 1
+    in bits 16 + 4p.  ``scales`` and ``zeros`` (or None: 8) are ``[ceil(in / group), rows]``
+    in the activations' dtype.  from_codes and quantize make them."""
 
-    def __init__(self, codes, scales, zeros, in_features, group_size):
+    def __init__(self, codes, scales, zeros, out_features, in_features, group_size):
         _check_group(group_size)
-        words, groups = -(-in_features // 128) * 16, -(-in_features // group_size)
-        if codes.dtype != torch.int32 or codes.dim() != 2 or codes.shape[1] != words:
-            raise ValueError(f"codes must be int32 [out, {words}]")
-        if scales.dtype not in _DTYPES or scales.shape != (groups, codes.shape[0]):
-            raise ValueError(f"scales must be fp32, bf16 or fp16 [{groups}, {codes.shape[0]}]")
+        groups, rows = -(-in_features // group_size), -(-out_features // 16) * 16
+        shape = (rows // 16, -(-in_features // 128), 64, 4)
+        if min(out_features, in_features) < 1 or codes.dtype != torch.int32 or codes.shape != shape:
+            raise ValueError(f"codes must be int32 {list(shape)}")
+        if scales.dtype not in _DTYPES or scales.shape != (groups, rows):
+            raise ValueError(f"scales must be fp32, bf16 or fp16 [{groups}, {rows}]")
         if zeros is not None and (zeros.dtype != scales.dtype or zeros.shape != scales.shape):
             raise ValueError("zeros must have the scales' dtype and shape")
         for t in (scales, zeros):
             if t is not None and t.device != codes.device:
                 raise RuntimeError("codes, scales and zeros must be on one device")
-        self.codes, self.scales = codes.contiguous(), scales.detach().resolve_neg().contiguous()
-        self.zeros = None if zeros is None else zeros.detach().resolve_neg().contiguous()
-        if self.codes.data_ptr() % 16:
-            self.codes = self.codes.clone()
-        self.in_features, self.out_features = int(in_features), codes.shape[0]
+        self.codes, self.scales = _aligned(codes), _aligned(scales)
+        self.zeros = None if zeros is None else _aligned(zeros)
+        self.in_features, self.out_features = int(in_features), int(out_features)
         self.group_size = int(group_size)
 
     @classmethod
@@ -56,12 +65,14 @@ class Int4Weight:
         shape = (out, -(-k // group_size))
         if scales.shape != shape or (zeros is not None and zeros.shape != shape):
             raise ValueError(f"scales and zeros must be {list(shape)}")
-        c = codes.to(torch.int32) & 15
-        c = nn.functional.pad(c, (0, -(-k // 128) * 128 - k)).view(out, -1, 8)
-        bits = torch.tensor([0, 16, 4, 20, 8, 24, 12, 28], dtype=torch.int32, device=codes.device)
-        words = (c << bits).sum(-1, dtype=torch.int32)  # disjoint bits; the sign bit wraps into place
-        z = None if zeros is None else zeros.to(scales.dtype).t().contiguous()
-        return cls(words, scales.t().contiguous(), z, k, group_size)
+        pad = -out % 16
+        c = nn.functional.pad(codes.to(torch.int32) & 15, (0, -k % 128, 0, pad))
+        bits = torch.tensor(_BITS, dtype=torch.int32, device=codes.device)
+        # disjoint bits (the last's sign wraps into place); [tile, i, block, j, r] to [tile, block, r, i, j]
+        words = (c.view((out + pad) // 16, 16, -1, 4, 4, 8) << bits).sum(-1, dtype=torch.int32).permute(0, 2, 4, 1, 3)
+        s, z = (None if t is None else nn.functional.pad(t.to(scales.dtype), (0, 0, 0, pad)).t().contiguous()
+                for t in (scales, zeros))
+        return cls(words.reshape(words.shape[0], -1, 64, 4), s, z, out, k, group_size)
 
     @classmethod
     def quantize(cls, weight, group_size=128, zero_points=False, dtype=None):
@@ -91,11 +102,13 @@ class Int4Weight:
 
     def dequantize(self):
         """The fp32 ``[out, in]`` matrix this stands for."""
-        bits = torch.tensor([0, 16, 4, 20, 8, 24, 12, 28], dtype=torch.int32, device=self.codes.device)
-        c = ((self.codes[..., None] >> bits) & 15).flatten(1)[:, :self.in_features].float()
+        bits = torch.tensor(_BITS, dtype=torch.int32, device=self.codes.device)
+        tiles, blocks = self.codes.shape[:2]
+        c = (self.codes.view(tiles, blocks, 4, 16, 4).permute(0, 3, 1, 4, 2)[..., None] >> bits) & 15
+        c = c.reshape(16 * tiles, -1)[:, :self.in_features].float()
         group = torch.arange(self.in_features, device=c.device) // self.group_size
         zero = 8.0 if self.zeros is None else self.zeros.float()[group].t()
-        return (c - zero) * self.scales.float()[group].t()
+        return ((c - zero) * self.scales.float()[group].t())[:self.out_features]
 
 
 def int4_linear(x, weight: Int4Weight):
@@ -107,8 +120,8 @@ def int4_linear(x, weight: Int4Weight):
     infinity gives NaN."""
     # the plain case runs in native code (csrc/ca_torch.cpp); what it does not take is checked here
     if x.is_cuda and not torch.compiler.is_compiling():
-        y = _native.torch_ext().int4(x, weight.codes, weight.scales, weight.zeros, weight.in_features,
-                                     weight.group_size)
+        y = _native.torch_ext().int4(x, weight.codes, weight.scales, weight.zeros, weight.out_features,
+                                     weight.in_features, weight.group_size)
         if y is not None:
             return y
     if torch.is_grad_enabled() and x.requires_grad:
@@ -156,7 +169,7 @@ class Int4Linear(nn.Module):
         return cls(Int4Weight.quantize(linear.weight, group_size, zero_points, dtype))
 
     def forward(self, x):
-        w = Int4Weight(self.codes, self.scales, self.zeros, self.in_features, self.group_size)
+        w = Int4Weight(self.codes, self.scales, self.zeros, self.out_features, self.in_features, self.group_size)
         return int4_linear(x.to(self.scales.dtype), w)
 
 

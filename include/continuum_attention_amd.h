@@ -372,9 +372,11 @@ int ca_rotary_append(const ca_rotary* r, const void* v, long long v_token_stride
 
 /* y[m][n] = sum_k x[m][k] scales[k / group][n] (code[n][k] - zeros[k / group][n]),
  * zeros NULL: 8.  x, y, scales and zeros of `dtype`; rows of x and y x_stride and
- * y_stride elements apart, scales and zeros [ceil(K / group)][N].  codes: [N] rows
- * of ceil(K / 128) * 16 words of 32 bits, 16-byte aligned; word w holds columns
- * 8w .. 8w + 7, column 8w + 2p in bits 4p and 8w + 2p + 1 in bits 16 + 4p.  group is
+ * y_stride elements apart.  With N rounded up to a multiple of 16, N16, scales and
+ * zeros are [ceil(K / group)][N16], and codes [N16 / 16][ceil(K / 128)] tiles of 16 rows
+ * by 128 columns: 64 times 4 words of 32 bits, words (16r + i, j) holding row i,
+ * columns c = 32j + 8r .. c + 7, column c + 2p in bits 4p and c + 2p + 1 in bits 16 + 4p.
+ * All 16-byte aligned; what lies past N and K is finite and has no effect.  group is
  * 32, 64 or a multiple of 128.  An infinity in a row of x gives NaN there. */
 int ca_int4_linear(const void* x, long long x_stride, const unsigned* codes, const void* scales,
                    const void* zeros, void* y, long long y_stride, int dtype, int M, int N, int K,

@@ -194,8 +194,8 @@ def test_int4_on_the_cpu_and_refusals(ca):
     for fn, match in ((lambda: ca.Int4Weight.from_codes(codes, scales, zeros, 48), "groups"),
                       (lambda: ca.Int4Weight.from_codes(codes.float(), scales, zeros, 32), "integers"),
                       (lambda: ca.Int4Weight.from_codes(codes, scales[:, :2], None, 32), "scales"),
-                      (lambda: ca.Int4Weight(w.codes[:, :3], w.scales, None, 77, 32), "codes"),
-                      (lambda: ca.Int4Weight(w.codes, w.scales.double(), None, 77, 32), "scales"),
+                      (lambda: ca.Int4Weight(w.codes[:, :, :3], w.scales, None, 10, 77, 32), "codes"),
+                      (lambda: ca.Int4Weight(w.codes, w.scales.double(), None, 10, 77, 32), "scales"),
                       (lambda: ca.int4_linear(x[:, :70], w), "columns"),
                       (lambda: ca.int4_linear(x.bfloat16(), w), "scales are")):
         with pytest.raises(ValueError, match=match):
