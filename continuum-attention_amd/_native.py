@@ -93,7 +93,7 @@ SIGNATURES = {
     "ca_bf16_shadow": (_i, [_vp, _i, _vp, _i, _vp]),
     "ca_swiglu_fwd_f32": (_i, [_vp, _vp, _i, _i, _vp]),
     "ca_swiglu_bwd_f32": (_i, [_vp, _vp, _vp, _i, _i, _vp]),
-    "ca_paged_attention_workspace_bytes": (_sz, [_i] * 8),
+    "ca_paged_attention_workspace_bytes": (_sz, [_i] * 9),
     "ca_paged_attention": (_i, [_cache_p, _vp, _ll, _ll, _i, _vp, _vp, _ll, _ll, _vp, _ll, _ll, _i,
                                 _i, _i, _vp, _sz, _vp]),
     "ca_evict": (_i, [_cache_p, _vp, _ll, _ll, _i, _i, _i, _i, _vp, _ll, _vp, _vp, _vp, _vp]),

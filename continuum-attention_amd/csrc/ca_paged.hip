@@ -255,6 +255,37 @@ __device__ __forceinline__ void span_weights(const float (&s)[8], float sl, floa
   }
 }
 
+// The weights of the eight keys before the lane's scores' (key skey - 1 + r in
+// w[r], skey the key of s[0]) but for the right share that w[0] gets from its own
+// segment; returns the one that the key of s[7] gets.  sl: the score of w[0]'s key.
+template <bool MASK>
+__device__ __forceinline__ float shared_weights(const float (&s)[8], float sl, int skey, int pos, float (&w)[8]) {
+  float pl = fast_exp2(sl), from_left = 0.f;
+#pragma unroll
+  for (int r = 0; r < 8; ++r) {
+    const float sr = s[r];
+    const float pr = fast_exp2(sr);
+    float L, R;
+    seg_shares(sl, sr, pl, pr, L, R);
+    const int key = skey + r;
+    if (MASK) {
+      const bool ok = key <= pos;
+      L = ok ? L : 0.f;
+      R = ok ? R : 0.f;
+    }
+    w[r] = L + from_left;
+    if (MASK) {
+      const float cap = 2.0f * pl;
+      w[r] += key == 1 && pos >= 0 ? cap : 0.f;
+      w[r] += key - 1 == pos && pos >= 0 ? cap : 0.f;
+    }
+    from_left = R;
+    sl = sr;
+    pl = pr;
+  }
+  return from_left;
+}
+
 // One wave's running softmax: shift (log2 units, whole), sum of weights (this
 // lane's part) and O^T, whose lane holds columns 16 b + 4 G4 + e of its query.
 template <int DT> struct Running {
@@ -375,6 +406,29 @@ __device__ __forceinline__ void add_values_seen(Running<DT>& st, const E* vs, co
     }
 }
 
+// The same in fp32 with V from memory (shared memory holds limbs of the finite ones).
+template <int DT>
+__device__ __forceinline__ void add_specials(Running<DT>& st, const float* vh, const PagedCache& c,
+                                             const int* table, const float (&w)[8], int k0, int end, int pos,
+                                             int pos_max) {
+  const int lane = threadIdx.x & 63, i = lane & 15, G4 = lane >> 4;
+#pragma unroll
+  for (int r = 0; r < 8; ++r)
+    for (int g = 0; g < 4; ++g) {
+      const int key = k0 + 8 * g + r;
+      const float x = __shfl(w[r], 16 * g + i);
+      if (key >= end) continue;  // uniform
+      const float* v = vh + row_at(c, row_ref(c, table, key, pos_max));
+#pragma unroll
+      for (int b = 0; b < DT / 16; ++b) {
+        if (16 * b + 4 * G4 >= c.D) continue;
+        const f32x4 y = ld4(v + 16 * b + 4 * G4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) st.o[b][e] += key <= pos && !is_finite(y[e]) ? x * y[e] : 0.f;
+      }
+    }
+}
+
 __device__ __forceinline__ float nan_value() { return __int_as_float(0x7fc00000); }
 
 // Is a page number of slots [first, last] outside the cache?  (All threads of
@@ -387,14 +441,39 @@ __device__ __forceinline__ bool bad_pages(const PagedCache& c, const int* table,
   return __syncthreads_or(bad);
 }
 
-// Many rows: four waves of 16 rows each share the tiles of V, which they stage
-// two in turn.
-template <class E, int DT>
-__global__ __launch_bounds__(256) void ca_paged_attention_kernel(PagedAttnIO io) {
+// Many rows: WV waves of 16 rows each share the tiles of V.  A weight tile is the
+// 32 keys from k0 on, its score tile the 32 from k0 + 1 on (slot x of the scores
+// is key k0 + 1 + x): the segment that ends at a score's key gives its left share
+// to the weight in the same register and its right share to the next one, the
+// last one of a tile to the next tile, as in the training forward.  So nothing is
+// done twice but for the segment that crosses a split's start, which comes from
+// one product of its own.  Tiles start at multiples of 32, as for few rows.
+//
+// fp32 goes through three bf16 limbs here: K and V are split once for all of the
+// waves when they are staged, and six bf16 products take 40% of the time of one
+// on the fp32 instruction.
+template <class E, int DT, int WV> struct Many {
   typedef Tile<E, DT> P;
-  constexpr int kRows = 64;
-  constexpr int kV = (32 * P::kChunks + 255) / 256;  // 16-byte loads of a thread per tile of V
-  __shared__ __attribute__((aligned(16))) E vbuf[2 * 32 * P::kRow];
+  static constexpr int kThreads = 64 * WV, kRows = 16 * WV;
+  static constexpr int kChunks = 32 * P::kChunks;                       // 16-byte chunks of a tile
+  static constexpr int kLoads = (kChunks + kThreads - 1) / kThreads;   // of each thread
+  static constexpr int kLRow = DT + 16;                                 // staged row of bf16
+  static constexpr int kPlane = 32 * kLRow;
+  // V of two tiles; fp32: limb planes of K and V of two tiles
+  static constexpr int kBytes = 2 * (P::kF32 ? 6 * kPlane * 2 : 32 * P::kRow * 2);
+};
+
+// Waves per SIMD that the registers are held to: what fits without spilling.
+template <class E, int DT> constexpr int many_waves() {
+  return std::is_same<E, float>::value ? (DT <= 32 ? 4 : DT <= 64 ? 3 : 2) : DT <= 64 ? 4 : 2;
+}
+
+template <class E, int DT, int WV, bool PAGE32>
+__global__ __launch_bounds__(64 * WV, (many_waves<E, DT>())) void ca_paged_attention_kernel(PagedAttnIO io) {
+  typedef Tile<E, DT> P;
+  typedef Many<E, DT, WV> M;
+  constexpr int KS = DT / 32;  // 32-wide products of the scores in limbs
+  __shared__ __attribute__((aligned(16))) unsigned char lds[M::kBytes];
   __shared__ int special[2];  // tile (plus one) whose V holds a value that is not finite
 
   const PagedCache& c = io.c;
@@ -411,156 +490,316 @@ __global__ __launch_bounds__(256) void ca_paged_attention_kernel(PagedAttnIO io)
   const int* table = c.table + (long long)b * c.table_stride;
   const E* kh = static_cast<const E*>(c.k) + (long long)h * c.head_stride;
   const E* vh = static_cast<const E*>(c.v) + (long long)h * c.head_stride;
-  const int tiles = (rows + kRows - 1) / kRows;
+  const int row_tiles = (rows + M::kRows - 1) / M::kRows;
+  const int rs = (int)c.row_stride;  // (PAGE32: below 2^25)
 
   // longest rows first
-  for (int back = tile0; back < tiles; back += io.row_tiles) {
-    const int row0 = (tiles - 1 - back) * kRows;
-    const int last_row = row0 + kRows < rows ? row0 + kRows - 1 : rows - 1;
+  for (int back = tile0; back < row_tiles; back += io.row_tiles) {
+    const int row0 = (row_tiles - 1 - back) * M::kRows;
+    const int last_row = row0 + M::kRows < rows ? row0 + M::kRows - 1 : rows - 1;
     const int pos_max = sp.len - sp.n + last_row / io.group;  // last slot any row sees
     const int pos_min = sp.len - sp.n + row0 / io.group;
     const int first = split * io.split_keys;
-    if (pos_max < first) {
-      if (split > 0) continue;  // nothing here; row_splits() says so to the one who joins
-    }
-    const int end = split == io.splits - 1 ? pos_max + 1
-                    : first + io.split_keys < pos_max + 1 ? first + io.split_keys : pos_max + 1;
+    if (pos_max < first && split > 0) continue;  // nothing here; the join knows
+    const int end = split == io.splits - 1 || first + io.split_keys > pos_max ? pos_max + 1 : first + io.split_keys;
+    const int ntiles = end > first ? (end - first + 31) / 32 : 0;
+    // (fp32: the quarter rows feed the product at the split's start, the limbs the tiles)
     const Rows<E, DT> R = load_rows<E, DT>(io, sp, h, row0 + 16 * wave + i16);
+    Limbs qb[P::kF32 ? KS : 1];
+    if constexpr (P::kF32) {
+      const float* q = static_cast<const float*>(io.q);
+      if (R.row >= 0) q += (R.row / io.Hq) * io.q_ts + (R.row % io.Hq) * io.q_hs;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; e += 4) {
+          const int d = 32 * ks + 8 * G4 + e;
+          const f32x4 v = R.row >= 0 && d < c.D ? ld4(q + d) : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int f = 0; f < 4; ++f) x[e + f] = v[f];
+        }
+        qb[ks] = split8(x);
+      }
+    }
     Running<DT> st;
     st.m = kNegBig;
     st.z = 0.f;
 #pragma unroll
     for (int x = 0; x < DT / 16; ++x) st.o[x] = f32x4{0.f, 0.f, 0.f, 0.f};
     if (tid < 2) special[tid] = 0;
-    const int ntiles = end > first ? (end - first + kOwned - 1) / kOwned : 0;
     bool bad = false;
-    if (ntiles > 0) {
-      const int halo = end <= pos_max ? end : pos_max;
-      bad = bad_pages(c, table, first > 0 ? first - 1 : 0, halo);
-    } else {
-      __syncthreads();
-    }
+    if (ntiles > 0) bad = bad_pages(c, table, first > 0 ? first - 1 : 0, end <= pos_max ? end : pos_max);
+    else __syncthreads();
     if (bad) {
       st.m = st.z = nan_value();
-    } else {
-      KRows<E, DT> kr;
-      RowRef kref[2], vref[kV];
-      u32x4 vreg[kV];
-      auto refs = [&](int t) {  // page numbers of tile t's rows
-        const int key = first + t * kOwned - 1;
-#pragma unroll
-        for (int x = 0; x < 2; ++x) kref[x] = row_ref(c, table, key + k_slot(x), pos_max);
-#pragma unroll
-        for (int x = 0; x < kV; ++x)
-          vref[x] = row_ref(c, table, key + (tid + x * 256) / P::kChunks, pos_max);
+    } else if (ntiles > 0) {
+      // ---- where rows lie ----
+      auto clamped = [&](int key) { return key < 0 ? 0 : key > pos_max ? pos_max : key; };
+      auto page_at = [&](int key) { return table[page_of(c.div, clamped(key))]; };
+      // of a key whose page's number is known
+      auto in_page = [&](int key, int page) {
+        const int at = clamped(key), idx = page_of(c.div, at);
+        return (long long)__builtin_amdgcn_readfirstlane(page) * c.page_stride +
+               (long long)(at - idx * (int)c.div.size) * c.row_stride;
       };
-      auto load_v = [&](int t) {
-        const int key = first + t * kOwned - 1;
+      int page0 = 0, page1 = 0;  // PAGE32: of the tile to be loaded next, and of the one behind it
+      RowRef kref[P::kF32 ? M::kLoads : 2], vref[M::kLoads];
+      auto look_up = [&](int k0) {  // of the tile to be loaded next
+        if constexpr (PAGE32) {
+          page0 = page1;
+          page1 = page_at(k0 + 32);
+        } else {
 #pragma unroll
-        for (int x = 0; x < kV; ++x) {
-          const int u = tid + x * 256, row = u / P::kChunks, d = u % P::kChunks * P::kVec;
-          // rows of other tiles and behind the last key stay out: zeros
-          const bool mine = row > 0 && row < 31 && key + row < end && d < c.D;
-          vreg[x] = mine ? *reinterpret_cast<const u32x4*>(vh + row_at(c, vref[x]) + d) : u32x4{0, 0, 0, 0};
+          for (int x = 0; x < (P::kF32 ? M::kLoads : 2); ++x)
+            kref[x] = row_ref(c, table, k0 + 1 + (P::kF32 ? (tid + x * M::kThreads) / P::kChunks : k_slot(x)), pos_max);
+#pragma unroll
+          for (int x = 0; x < M::kLoads; ++x)
+            vref[x] = row_ref(c, table, k0 + (tid + x * M::kThreads) / P::kChunks, pos_max);
         }
       };
-      auto store_v = [&](int t, int buf) {
-        const bool look = first + t * kOwned + 30 > pos_min;
+      // ---- loads of a tile ----
+      KRows<E, DT> kr;                // 16-bit: the wave's operand
+      u32x4 kreg[M::kLoads], vreg[M::kLoads];  // what this thread stages (kreg: fp32)
+      auto load_tile = [&](int k0) {
+        long long at0 = 0, at1 = 0;
+        if constexpr (PAGE32) {
+          at0 = in_page(k0, page0);
+          at1 = in_page(k0 + 32, page1);
+        }
+        if constexpr (!P::kF32) {
+          const int d0 = DT / 4 * G4;
 #pragma unroll
-        for (int x = 0; x < kV; ++x) {
-          const int u = tid + x * 256, row = u / P::kChunks, d = u % P::kChunks * P::kVec;
-          if ((32 * P::kChunks) % 256 == 0 || row < 32) {
-            *reinterpret_cast<u32x4*>(vbuf + (buf * 32 + row) * P::kRow + d) = vreg[x];
+          for (int x = 0; x < 2; ++x) {
+            const E* p;
+            if constexpr (PAGE32)
+              p = kh + (k_slot(x) == 31 ? at1 + d0 : at0 + ((k_slot(x) + 1) * rs + d0));
+            else
+              p = kh + row_at(c, kref[x]) + d0;
+#pragma unroll
+            for (int j = 0; j < P::kPieces; ++j)
+              kr.k[x][j] = d0 + P::kVec * j < c.D ? *reinterpret_cast<const u32x4*>(p + P::kVec * j) : u32x4{0, 0, 0, 0};
+          }
+        }
+        const bool whole = k0 + 32 <= end;
+#pragma unroll
+        for (int x = 0; x < M::kLoads; ++x) {
+          const int u = tid + x * M::kThreads, row = u / P::kChunks, d = u % P::kChunks * P::kVec;
+          // V: keys behind the last one stay out: zeros
+          const bool mine = row < 32 && d < c.D && (whole || k0 + row < end);
+          const E* p;
+          if constexpr (PAGE32) p = vh + at0 + (row * rs + d);
+          else p = vh + row_at(c, vref[x]) + d;
+          vreg[x] = mine ? *reinterpret_cast<const u32x4*>(p) : u32x4{0, 0, 0, 0};
+          if constexpr (P::kF32) {
+            if constexpr (PAGE32) p = kh + (row == 31 ? at1 + d : at0 + ((row + 1) * rs + d));
+            else p = kh + row_at(c, kref[x]) + d;
+            kreg[x] = row < 32 && d < c.D ? *reinterpret_cast<const u32x4*>(p) : u32x4{0, 0, 0, 0};
+          }
+        }
+      };
+      auto stage = [&](int t, int buf) {
+        const bool look = first + 32 * (t + 1) > pos_min;
+#pragma unroll
+        for (int x = 0; x < M::kLoads; ++x) {
+          const int u = tid + x * M::kThreads, row = u / P::kChunks, d = u % P::kChunks * P::kVec;
+          if (M::kChunks % M::kThreads != 0 && row >= 32) continue;
+          if constexpr (P::kF32) {
+            __bf16* kp = reinterpret_cast<__bf16*>(lds) + buf * 6 * M::kPlane;
+            const f32x4 kv = __builtin_bit_cast(f32x4, kreg[x]);
+            f32x4 vv = __builtin_bit_cast(f32x4, vreg[x]);
+            bool odd = false;
+            if (look) {
+              // values that are not finite stay out of the limbs, for the rows
+              // that see them to add by themselves
+#pragma unroll
+              for (int e = 0; e < 4; ++e) odd = odd || !is_finite(vv[e]);
+              if (odd) special[buf] = t + 1;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) vv[e] = is_finite(vv[e]) ? vv[e] : 0.f;
+            }
+            unsigned k0w[3], k1w[3], v0w[3], v1w[3];
+            split_pair_limbs<3>(kv[0], kv[1], k0w);
+            split_pair_limbs<3>(kv[2], kv[3], k1w);
+            split_pair_limbs<3>(vv[0], vv[1], v0w);
+            split_pair_limbs<3>(vv[2], vv[3], v1w);
+#pragma unroll
+            for (int l = 0; l < 3; ++l) {
+              *reinterpret_cast<u32x2*>(kp + l * M::kPlane + row * M::kLRow + d) = u32x2{k0w[l], k1w[l]};
+              *reinterpret_cast<u32x2*>(kp + (3 + l) * M::kPlane + row * M::kLRow + d) = u32x2{v0w[l], v1w[l]};
+            }
+          } else {
+            *reinterpret_cast<u32x4*>(reinterpret_cast<E*>(lds) + (buf * 32 + row) * P::kRow + d) = vreg[x];
             if (look && any_special(vreg[x], (const E*)nullptr)) special[buf] = t + 1;
           }
         }
       };
-      if (ntiles > 0) {
-        refs(0);
-        load_k<E, DT>(c, kh, kref, kr);
-        load_v(0);
-        refs(1);
-        store_v(0, 0);
-        __syncthreads();
-      }
-      for (int t = 0; t < ntiles; ++t) {
-        const int buf = t & 1;
-        const int key = first + t * kOwned - 1;  // key of slot 0
-        float s[8], w[8];
-        tile_products<E, DT>(kr, R, s);
-        if (t + 1 < ntiles) {
-          load_k<E, DT>(c, kh, kref, kr);
-          load_v(t + 1);
-          refs(t + 2);
+
+      // ---- the split's start: the scores of its first key and of the one before ----
+      // Scores are kept relative to shift = m + kAbove (see tile_weights).
+      constexpr float kAbove = kShareShift - weight_octaves<E>();
+      float shift, s_carry, r_carry = 0.f;  // score of the tile's first key, right share it gets
+      {
+        const int key = (i16 & 3) == 1 ? first - 1 : first;
+        const RowRef ref = row_ref(c, table, key, pos_max);
+        const E* p = kh + row_at(c, ref) + DT / 4 * G4;
+        f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+        if constexpr (PAGE32) page1 = page_at(first);
+        look_up(first);
+        load_tile(first);
+#pragma unroll
+        for (int j = 0; j < P::kPieces; ++j) {
+          const bool in = DT / 4 * G4 + P::kVec * j < c.D;
+          const u32x4 k = in ? *reinterpret_cast<const u32x4*>(p + P::kVec * j) : u32x4{0, 0, 0, 0};
+          if constexpr (P::kF32) {
+            const f32x4 a = __builtin_bit_cast(f32x4, k), q = __builtin_bit_cast(f32x4, R.q[j]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc = mfma16_f32(a[e], q[e], acc);
+          } else {
+            acc = mfma16_of(k, R.q[j], acc, (const E*)nullptr);
+          }
         }
-        const int key0 = key + 8 * G4;
-        const bool mask = key < 0 || key + 31 > pos_min;
+        const float at = acc[0] * R.scale, before = acc[1] * R.scale;
+        const bool sees = first <= R.pos, seg = sees && first > 0;
+        // (rows that see nothing yet never will in this split; from a score that
+        // is not finite no shift can start)
+        const float top = seg ? fmaxf(at, before) : at;
+        shift = (sees && is_finite(top) ? rintf(top) : 0.f) + kAbove;
+        s_carry = at - shift;
+        const float sl = before - shift;
+        float L, Rs;
+        seg_shares(sl, s_carry, fast_exp2(sl), fast_exp2(s_carry), L, Rs);
+        r_carry = seg ? Rs : 0.f;
+        stage(0, 0);
+        if (ntiles > 1) look_up(first + 32);
+      }
+      __syncthreads();
+
+      for (int t = 0; t < ntiles; ++t) {
+        const int buf = t & 1, k0 = first + 32 * t;
+        float s[8], w[8];
+        if constexpr (P::kF32) {
+          const __bf16* kp = reinterpret_cast<const __bf16*>(lds) + buf * 6 * M::kPlane;
+          f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) {
+            Limbs ka[2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) ka[x] = limbs_at<3>(kp + k_slot(x) * M::kLRow + 32 * ks + 8 * G4, M::kPlane);
+#pragma unroll
+            for (int step = 0; step < 6; ++step) {
+              acc[0] = mfma16_step(step, ka[0], qb[ks], acc[0]);
+              acc[1] = mfma16_step(step, ka[1], qb[ks], acc[1]);
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < 8; ++r) s[r] = acc[r >> 2][r & 3];
+        } else {
+          tile_products<E, DT>(kr, R, s);
+        }
+        if (t + 1 < ntiles) {
+          load_tile(k0 + 32);
+          if (t + 2 < ntiles) look_up(k0 + 64);
+        }
+        const int skey = k0 + 1 + 8 * G4;  // key of s[0]; w[0]'s is the one before
+        const bool mask = k0 == 0 || k0 + 32 > pos_min;
+        // relative to the shift so far, which a tile seldom moves
         float mt = kNegBig;
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
-          s[r] *= R.scale;
-          mt = fmaxf(mt, !mask || (key0 + r >= 0 && key0 + r <= R.pos) ? s[r] : kNegBig);
+          s[r] = fmaf(s[r], R.scale, -shift);
+          mt = fmaxf(mt, !mask || skey + r <= R.pos ? s[r] : kNegBig);
         }
         mt = rows_max(mt);
-        const bool grow = mt > st.m + kLazyRescale;
+        const bool grow = mt > kLazyRescale - kAbove;
         if (wave_any(grow)) {
-          const float m = grow ? rintf(mt) : st.m;
-          const float alpha = grow ? fast_exp2(st.m - m) : 1.0f;
+          const float up = grow ? rintf(mt + kAbove) : 0.f;
+          const float alpha = fast_exp2(-up);
 #pragma unroll
           for (int x = 0; x < DT / 16; ++x) st.o[x] *= alpha;
           st.z *= alpha;
-          st.m = m;
-        }
-        const float shift = st.m + (kShareShift - weight_octaves<E>());
+          r_carry *= alpha;
+          s_carry -= up;
+          shift += up;
 #pragma unroll
-        for (int r = 0; r < 8; ++r) s[r] -= shift;
-        if (mask) tile_weights<true>(s, key0, R.pos, w);
-        else tile_weights<false>(s, key0, R.pos, w);
+          for (int r = 0; r < 8; ++r) s[r] -= up;
+        }
+        const float s_last = row_before(s[7]);  // lane row 0: the next tile's carry
+        const float sl0 = G4 == 0 ? s_carry : s_last;
+        s_carry = s_last;
+        float r_out = mask ? shared_weights<true>(s, sl0, skey, R.pos, w) : shared_weights<false>(s, sl0, skey, R.pos, w);
+        r_out = row_before(r_out);
+        w[0] += G4 == 0 ? r_carry : r_out;
+        r_carry = r_out;
 #pragma unroll
         for (int r = 0; r < 8; ++r) st.z += w[r];
-        const E* vs = vbuf + buf * 32 * P::kRow;
-        Limbs16<E> wl;
-        if constexpr (!P::kF32) wl = limbs16<E>(w);
-        if (mask && special[buf] == t + 1) {
-          add_values<E, DT, true>(st, vs, w, wl);
-          add_values_seen<E, DT>(st, vs, w, key, R.pos, 1, 31);
+        if constexpr (P::kF32) {
+          const __bf16* vp = reinterpret_cast<const __bf16*>(lds) + (buf * 6 + 3) * M::kPlane;
+          const __bf16* base = vp + (8 * G4 + (i16 >> 2)) * M::kLRow + 4 * (i16 & 3);
+          const Limbs wb = split8(w);
+#pragma unroll
+          for (int x = 0; x < DT / 16; x += 2) {
+            f32x4 part[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+            Limbs va[2];
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              const __bf16* at = base + 16 * (x + y);
+              va[y].h = lds_read_tr8(at, at + 4 * M::kLRow);
+              va[y].m = lds_read_tr8(at + M::kPlane, at + M::kPlane + 4 * M::kLRow);
+              va[y].l = lds_read_tr8(at + 2 * M::kPlane, at + 2 * M::kPlane + 4 * M::kLRow);
+            }
+#pragma unroll
+            for (int step = 0; step < 6; ++step) {
+              part[0] = mfma16_step(step, va[0], wb, part[0]);
+              part[1] = mfma16_step(step, va[1], wb, part[1]);
+            }
+            // a tile's product is added once: its rounding does not grow with the sum
+            st.o[x] += part[0];
+            st.o[x + 1] += part[1];
+          }
+          if (mask && special[buf] == t + 1) add_specials<DT>(st, vh, c, table, w, k0, end, R.pos, pos_max);
         } else {
-          add_values<E, DT, false>(st, vs, w, wl);
+          const Limbs16<E> wl = limbs16<E>(w);
+          const E* vs = reinterpret_cast<const E*>(lds) + buf * 32 * P::kRow;
+          if (mask && special[buf] == t + 1) {
+            add_values<E, DT, true>(st, vs, w, wl);
+            add_values_seen<E, DT>(st, vs, w, k0, R.pos, 0, 32);
+          } else {
+            add_values<E, DT, false>(st, vs, w, wl);
+          }
         }
-        if (t + 1 < ntiles) store_v(t + 1, buf ^ 1);
+        if (t + 1 < ntiles) stage(t + 1, buf ^ 1);
         __syncthreads();
       }
       st.z = rows_sum(st.z);
+      st.m = first <= R.pos ? shift - kAbove : kNegBig;
     }
 
     const long long nrows = (long long)io.tokens * io.Hq;
-    {
-      const float meff = st.m - weight_octaves<E>();
-      if (R.row >= 0) {
-        if (io.splits == 1) {
-          const float inv = st.z == 0.f ? 0.f : 1.0f / st.z;
-          const int r = row0 + 16 * wave + i16, t = r / io.group, head = h * io.group + r - t * io.group;
-          E* o = static_cast<E*>(io.out) + (long long)(sp.t0 + t) * io.o_ts + (long long)head * io.o_hs;
+    const float meff = st.m - weight_octaves<E>();
+    if (R.row >= 0) {
+      if (io.splits == 1) {
+        const float inv = st.z == 0.f ? 0.f : 1.0f / st.z;
+        E* o = static_cast<E*>(io.out) + (R.row / io.Hq) * io.o_ts + (R.row % io.Hq) * io.o_hs;
 #pragma unroll
-          for (int x = 0; x < DT / 16; ++x)
-            if (16 * x + 4 * G4 < c.D) st4(o + 16 * x + 4 * G4, st.o[x] * inv);
-          if (io.stats && G4 == 0) {
-            io.stats[2 * R.row] = meff;
-            io.stats[2 * R.row + 1] = inv;
-          }
-        } else {
-          float* o = io.part_o + (split * nrows + R.row) * c.D;
+        for (int x = 0; x < DT / 16; ++x)
+          if (16 * x + 4 * G4 < c.D) st4(o + 16 * x + 4 * G4, st.o[x] * inv);
+        if (io.stats && G4 == 0) {
+          io.stats[2 * R.row] = meff;
+          io.stats[2 * R.row + 1] = inv;
+        }
+      } else {
+        float* o = io.part_o + (split * nrows + R.row) * c.D;
 #pragma unroll
-          for (int x = 0; x < DT / 16; ++x)
-            if (16 * x + 4 * G4 < c.D) st4(o + 16 * x + 4 * G4, st.o[x]);
-          if (G4 == 0) {
-            io.part_ml[2 * (split * nrows + R.row)] = meff;
-            io.part_ml[2 * (split * nrows + R.row) + 1] = st.z;
-          }
+        for (int x = 0; x < DT / 16; ++x)
+          if (16 * x + 4 * G4 < c.D) st4(o + 16 * x + 4 * G4, st.o[x]);
+        if (G4 == 0) {
+          io.part_ml[2 * (split * nrows + R.row)] = meff;
+          io.part_ml[2 * (split * nrows + R.row) + 1] = st.z;
         }
       }
-      __syncthreads();
     }
+    __syncthreads();  // the next row tile stages over this one's
   }
 }
 
@@ -1019,15 +1258,17 @@ __global__ __launch_bounds__(256) void ca_paged_sums_kernel(PagedAttnIO io) {
   }
 }
 
-template <class E, int DT>
+template <class E, int DT, bool PAGE32>
 hipError_t run_attention(const PagedAttnIO& io, hipStream_t s) {
-  const dim3 grid((unsigned)((long long)io.c.batch * io.c.heads * io.splits * io.row_tiles)), block(256);
-  if (io.tile_group == 0)
-    hipLaunchKernelGGL((ca_paged_attention_kernel<E, DT>), grid, block, 0, s, io);
-  else if (io.c.div.size % 32 == 0 && io.c.row_stride < 1 << 25)  // offsets within a tile in 32 bits
-    hipLaunchKernelGGL((ca_paged_few_kernel<E, DT, true>), grid, block, 0, s, io);
+  const dim3 grid((unsigned)((long long)io.c.batch * io.c.heads * io.splits * io.row_tiles));
+  if (io.tile_group)
+    hipLaunchKernelGGL((ca_paged_few_kernel<E, DT, PAGE32>), grid, dim3(256), 0, s, io);
+  else if (io.waves == 2)
+    hipLaunchKernelGGL((ca_paged_attention_kernel<E, DT, 2, PAGE32>), grid, dim3(128), 0, s, io);
+  else if (io.waves == 4)
+    hipLaunchKernelGGL((ca_paged_attention_kernel<E, DT, 4, PAGE32>), grid, dim3(256), 0, s, io);
   else
-    hipLaunchKernelGGL((ca_paged_few_kernel<E, DT, false>), grid, block, 0, s, io);
+    hipLaunchKernelGGL((ca_paged_attention_kernel<E, DT, 8, PAGE32>), grid, dim3(512), 0, s, io);
   return hipGetLastError();
 }
 template <class E, int DT>
@@ -1066,7 +1307,11 @@ template <class F> hipError_t by_type(int dtype, int D, F f) {
 
 hipError_t launch_paged_attention(const PagedAttnIO& io, int dtype, hipStream_t s) {
   return by_type(dtype, io.c.D, [&](auto width, auto* e) {
-    return run_attention<std::remove_pointer_t<decltype(e)>, decltype(width)::value>(io, s);
+    typedef std::remove_pointer_t<decltype(e)> E;
+    constexpr int kWidth = decltype(width)::value;
+    // pages that tiles of 32 keys never cross; offsets within a tile in 32 bits
+    const bool page32 = io.c.div.size % 32 == 0 && io.c.row_stride < 1 << 25;
+    return page32 ? run_attention<E, kWidth, true>(io, s) : run_attention<E, kWidth, false>(io, s);
   });
 }
 hipError_t launch_paged_combine(const PagedAttnIO& io, int dtype, hipStream_t s) {

@@ -4,6 +4,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <vector>
 
 #include "ca_evict.h"
 #include "ca_int4.h"
@@ -72,49 +73,107 @@ ca::PagedCache kernel_cache(const ca_paged_cache& c) {
 // How the attention's grid is cut.  max_new and max_length only size it: the
 // kernels read what is there from the device and walk all of it.
 struct AttnPlan {
-  int row_tiles, splits, split_keys, row_log, tile_group;
+  int row_tiles, splits, split_keys, row_log, tile_group, waves;
 };
-constexpr int kFewRows = 16;         // rows per key head that share a wave's columns
-constexpr int kTargetGroups = 2048;  // eight work groups for each of 256 CUs
-// with so many row tiles the device is full and partial sums cost more than
-// they even out: [2,2048] fp32 prompts in two splits 355 against 310 us
-constexpr int kEnoughGroups = 1024;
-constexpr int kLeastTiles = 8;       // tiles of a split (many rows)
+constexpr int kFewRows = 16;  // rows per key head that share a wave's columns
+constexpr int kCus = 256;
 constexpr int kMostSplits = 128;
 
 size_t partial_bytes(int splits, int tokens, int heads, int D) {
   return splits > 1 ? (size_t)splits * tokens * heads * (D + 2) * sizeof(float) : 0;
 }
-AttnPlan attn_plan(int batch, int kv_heads, int heads, int D, int tokens, int max_new, int max_length) {
-  const long long rows = (long long)std::max(1, std::min(max_new, tokens)) * (heads / kv_heads);
+
+// Many rows: the time, in steps of one tile of one work group, that `slots` work
+// groups at once take for row tiles of given lengths (in tiles, longest first, each
+// `slices` times) cut at `cut`: each item goes to the slot that is free first.
+int dealt_steps(int cut, const std::vector<int>& lengths, long long slices, long long slots) {
+  std::vector<long long> free_at(64, 0);  // slots that become free at each step
+  free_at[0] = slots;
+  size_t lo = 0, most = 0;
+  auto deal = [&](long long n, int steps) {
+    while (n > 0) {
+      while (free_at[lo] == 0) ++lo;
+      const long long k = std::min(n, free_at[lo]);
+      const size_t end = lo + steps;
+      free_at[lo] -= k;
+      if (end >= free_at.size()) free_at.resize(2 * end, 0);
+      free_at[end] += k;
+      most = std::max(most, end);
+      n -= k;
+    }
+  };
+  for (int len : lengths)
+    for (int at = 0; at < len; at += cut) deal(slices, std::min(cut, len - at));
+  return (int)most;
+}
+
+AttnPlan make_plan(int dtype, int batch, int kv_heads, int heads, int D, int tokens, int max_new, int max_length) {
+  const int group = heads / kv_heads;
+  const long long rows = (long long)std::max(1, std::min(max_new, tokens)) * group;
   const long long slices = (long long)batch * kv_heads;
+  const size_t cap = ca_workspace_cap();
   AttnPlan p;
-  int unit, least;  // keys that a split is a multiple of, and its least number of these
-  long long tiles;  // of rows
+  long long tiles = 1;  // of rows
+  int unit;             // keys that a split is a multiple of
+  long long splits;
   if (rows <= kFewRows) {
-    p.row_log = 0;
+    p.row_log = p.waves = 0;
     while ((1 << p.row_log) < rows) ++p.row_log;
-    tiles = 1;
     // tiles of keys that share a wave: as many as leave the device two waves on
     // each SIMD
     p.tile_group = kFewRows >> p.row_log;
     const long long key_tiles = std::max(1, (max_length + 31) / 32);
-    while (p.tile_group > 1 && slices * ((key_tiles + p.tile_group - 1) / p.tile_group) < kTargetGroups)
+    while (p.tile_group > 1 && slices * ((key_tiles + p.tile_group - 1) / p.tile_group) < 8 * kCus)
       p.tile_group >>= 1;
     unit = 32 * p.tile_group;
-    least = 4;  // one for each wave of a work group
+    // eight work groups for each CU (ragged lengths leave some empty: 32 tokens
+    // over up to 8192 slots 127 us with four, 116 with eight, 122 with 16), one
+    // group of tiles at least for each of their waves
+    const int units = std::max(1, (max_length + unit - 1) / unit);
+    splits = std::min<long long>(8 * kCus / slices, units / 4);
   } else {
     p.row_log = p.tile_group = 0;
-    tiles = (rows + 63) / 64;
-    unit = 30;
-    least = kLeastTiles;
+    p.waves = rows <= 32 ? 2 : rows <= 64 ? 4 : 8;
+    const int tile_rows = 16 * p.waves;
+    tiles = (rows + tile_rows - 1) / tile_rows;
+    unit = 32;
+    // By estimated time.  Work groups at once: those whose waves and shared memory
+    // fit; a step takes about 2 us per 64 columns with the device full, and a
+    // partial row 0.2 ns a column pair to write and read again.
+    const bool f32 = dtype == CA_DTYPE_F32;
+    const int simd_waves = D <= 32 ? 4 : D <= 64 ? (f32 ? 3 : 4) : 2;
+    long long per_cu = std::max(1, 4 * simd_waves / p.waves);
+    if (f32) per_cu = std::min<long long>(per_cu, D <= 32 ? 4 : D <= 64 ? 2 : 1);
+    const int key_tiles = std::max(1, (max_length + 31) / 32);
+    std::vector<int> lengths;  // of up to 64 row tiles (more are much alike)
+    const int shown = (int)std::min<long long>(tiles, 64);
+    for (int t = 0; t < shown; ++t) {
+      const long long last = std::min<long long>(rows, (tiles - t * tiles / shown) * tile_rows) - 1;
+      const long long keys = std::max<long long>(1, max_length - (rows - 1 - last) / group);
+      lengths.push_back((int)((keys + 31) / 32));
+    }
+    const long long copies = slices * tiles / shown;  // work groups per length
+    const double step_us = 0.55 * p.waves * per_cu / (simd_waves * 4) * 4 * std::max(1.0, D / 64.0) * (f32 ? 1.7 : 1.0);
+    double best = 0;
+    splits = 1;
+    if (copies > 0)
+      for (int s : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 24, 32, 48, 64}) {
+        if (s > 1 && key_tiles / s < 4) break;
+        const int cut = (key_tiles + s - 1) / s;
+        double us = step_us * dealt_steps(cut, lengths, copies, per_cu * kCus);
+        if (s > 1) {
+          double parts = 0;
+          for (int len : lengths) parts += (len + cut - 1) / cut;
+          us += 4 + parts / shown * slices * rows * D * 1.0e-4 / 64;
+        }
+        if (s == 1 || us < best) {
+          best = us;
+          splits = s;
+        }
+      }
   }
   const int units = std::max(1, (max_length + unit - 1) / unit);
-  long long splits = std::max<long long>(1, kTargetGroups / (slices * tiles));
-  if (!p.tile_group && slices * tiles >= kEnoughGroups) splits = 1;
-  splits = std::min<long long>(splits, std::max(1, units / least));
-  splits = std::min<long long>(splits, kMostSplits);
-  const size_t cap = ca_workspace_cap();
+  splits = std::max<long long>(1, std::min<long long>({splits, kMostSplits, units}));
   while (splits > 1 && cap && partial_bytes((int)splits, tokens, heads, D) > cap) --splits;
   const int per = (units + (int)splits - 1) / (int)splits;
   p.splits = (units + per - 1) / per;
@@ -123,16 +182,35 @@ AttnPlan attn_plan(int batch, int kv_heads, int heads, int D, int tokens, int ma
   p.row_tiles = (int)std::max<long long>(1, std::min<long long>(tiles, ((1ll << 31) - 1) / (slices * p.splits)));
   return p;
 }
+
+// The last plans of this thread: a decoder asks for the same ones layer after layer.
+AttnPlan attn_plan(int dtype, int batch, int kv_heads, int heads, int D, int tokens, int max_new, int max_length) {
+  struct Entry {
+    long long key[9];
+    AttnPlan plan;
+  };
+  static thread_local Entry kept[16];
+  static thread_local unsigned used = 0;
+  const long long key[9] = {dtype, batch, kv_heads, heads, D, tokens, max_new, max_length, (long long)ca_workspace_cap()};
+  for (unsigned i = 0; i < std::min(used, 16u); ++i)
+    if (std::equal(key, key + 9, kept[i].key)) return kept[i].plan;
+  Entry& e = kept[used++ % 16];
+  e.plan = make_plan(dtype, batch, kv_heads, heads, D, tokens, max_new, max_length);
+  std::copy(key, key + 9, e.key);
+  return e.plan;
+}
 size_t stats_bytes(int tokens, int heads) { return ((size_t)tokens * heads * 2 * sizeof(float) + 255) & ~(size_t)255; }
 
 }  // namespace
 
 extern "C" {
 
-size_t ca_paged_attention_workspace_bytes(int batch, int kv_heads, int heads, int head_dim, int tokens,
+size_t ca_paged_attention_workspace_bytes(int dtype, int batch, int kv_heads, int heads, int head_dim, int tokens,
                                           int max_new, int max_length, int with_sums) {
-  if (batch <= 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || head_dim <= 0 || tokens <= 0) return 0;
-  const AttnPlan p = attn_plan(batch, kv_heads, heads, head_dim, tokens, max_new, max_length);
+  if (batch <= 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || head_dim <= 0 || tokens <= 0 || max_new < 0 ||
+      max_length < 0 || max_length > kMaxSlots || (long long)batch * kv_heads > 1 << 24)
+    return 0;
+  const AttnPlan p = attn_plan(dtype, batch, kv_heads, heads, head_dim, tokens, max_new, max_length);
   return partial_bytes(p.splits, tokens, heads, head_dim) + (with_sums ? stats_bytes(tokens, heads) : 0);
 }
 
@@ -162,13 +240,14 @@ int ca_paged_attention(const ca_paged_cache* cache, const void* q, long long q_t
   if (max_new < 0 || max_length < 0 || sums_len < 0)
     return set_error(CA_ERR_INVALID, "%s: negative max_new, max_length or sums_len", op);
   max_length = std::min(max_length, cache->pages_per_seq * cache->page_size);
-  const size_t need = ca_paged_attention_workspace_bytes(cache->batch, cache->heads, heads, cache->head_dim,
-                                                         cache->tokens, max_new, max_length, sums != nullptr);
+  const size_t need = ca_paged_attention_workspace_bytes(cache->dtype, cache->batch, cache->heads, heads,
+                                                         cache->head_dim, cache->tokens, max_new, max_length, sums != nullptr);
   if (need && (!workspace || workspace_bytes < need))
     return set_error(CA_ERR_WORKSPACE, "%s: workspace of %zu bytes required, %zu given", op, need, workspace_bytes);
   if (!aligned(workspace, 16)) return set_error(CA_ERR_INVALID, "%s: workspace must be 16-byte aligned", op);
 
-  const AttnPlan p = attn_plan(cache->batch, cache->heads, heads, cache->head_dim, cache->tokens, max_new, max_length);
+  const AttnPlan p = attn_plan(cache->dtype, cache->batch, cache->heads, heads, cache->head_dim, cache->tokens, max_new,
+                               max_length);
   ca::PagedAttnIO io;
   io.c = kernel_cache(*cache);
   io.q = q;
@@ -199,6 +278,7 @@ int ca_paged_attention(const ca_paged_cache* cache, const void* q, long long q_t
   io.row_tiles = p.row_tiles;
   io.row_log = p.row_log;
   io.tile_group = p.tile_group;
+  io.waves = p.waves;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   hipError_t err = ca::launch_paged_attention(io, cache->dtype, s);
   if (err == hipSuccess && p.splits > 1) err = ca::launch_paged_combine(io, cache->dtype, s);

@@ -731,8 +731,8 @@ py::object attend(py::handle qo, py::handle kpo, py::handle vpo, py::handle tabl
     py::gil_scoped_release release;
     const c10::DeviceGuard guard(q.device());
     if (!out.defined()) out = empty(q.sizes(), q, q.scalar_type());
-    const size_t bytes = ca_paged_attention_workspace_bytes(c.batch, c.heads, (int)a.heads, c.head_dim, c.tokens,
-                                                            (int)max_new, (int)max_length, sums.defined());
+    const size_t bytes = ca_paged_attention_workspace_bytes(c.dtype, c.batch, c.heads, (int)a.heads, c.head_dim,
+                                                            c.tokens, (int)max_new, (int)max_length, sums.defined());
     Tensor ws;
     if (bytes) ws = workspace(bytes, q);
     check(ca_paged_attention(&c, q.const_data_ptr(), a.ts, a.hs, (int)a.heads, gain.const_data_ptr<float>(),

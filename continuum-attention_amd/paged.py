@@ -252,7 +252,7 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, starts, log_gain, 
         g = g.float().contiguous()
     sums = weight_sums if weight_sums is not None and weight_sums.numel() else None
     max_length = min(max_length, capacity)
-    nbytes = _workspace_bytes(c.batch, c.heads, H, D, N, max_new, max_length, int(sums is not None))
+    nbytes = _workspace_bytes(c.dtype, c.batch, c.heads, H, D, N, max_new, max_length, int(sums is not None))
     ws = torch.empty(max(nbytes, 1), device=dev, dtype=torch.uint8)
     with _native.on_device(dev):
         _native.check(_native.load().ca_paged_attention(

@@ -324,8 +324,8 @@ typedef struct {
  * of new tokens and cached length expected, size the grid and the workspace;
  * other numbers on the device give the same results.  A token that sees nothing
  * gets zeros; one that reads a table entry outside the cache gets NaN. */
-size_t ca_paged_attention_workspace_bytes(int batch, int kv_heads, int heads, int head_dim, int tokens,
-                                          int max_new, int max_length, int with_sums);
+size_t ca_paged_attention_workspace_bytes(int dtype, int batch, int kv_heads, int heads, int head_dim,
+                                          int tokens, int max_new, int max_length, int with_sums);
 int ca_paged_attention(const ca_paged_cache* cache, const void* q, long long q_token_stride,
                        long long q_head_stride, int heads, const float* log_gain, void* out,
                        long long out_token_stride, long long out_head_stride, float* sums,

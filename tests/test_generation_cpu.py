@@ -237,7 +237,7 @@ def test_c_abi_refusals(ca):
     assert attn(cache(), heads=3) == 1
     assert attn(cache(), q=p + 2) == 1 and attn(cache(), qs=(255, 64)) == 1 and attn(cache(), q=None) == 1
     assert attn(cache(), max_new=-1) == 1 and attn(cache(), gain=p + 1) == 1
-    need = lib.ca_paged_attention_workspace_bytes(2, 4, 4, 64, 3, 1, 100000, 0)
+    need = lib.ca_paged_attention_workspace_bytes(1, 2, 4, 4, 64, 3, 1, 100000, 0)
     assert need > 0
     c = cache(pages_per_seq=10000, table_stride=10000)
     assert attn(c, max_length=100000) == 3
