@@ -65,7 +65,7 @@ struct PagedAttnIO {
   int row_tiles;           // row tiles of the grid; work groups walk the rest
   // few rows: 2^row_log rows and tile_group tiles of 32 keys share a wave's 16
   // columns; tile_group 0: many rows, on `waves` waves (2, 4, 8) of 16
-  int row_log, tile_group, waves;
+  int row_log, tile_group, waves, tile_rows;
 };
 hipError_t launch_paged_attention(const PagedAttnIO& io, int dtype, hipStream_t s);
 hipError_t launch_paged_combine(const PagedAttnIO& io, int dtype, hipStream_t s);

@@ -65,6 +65,11 @@ __device__ __forceinline__ float row_behind(float x) {
   const float a = lane_xor16(x), b = lane_xor16(xhalf(x));
   return (threadIdx.x & 16) ? b : a;
 }
+// Value of the lane N places on in the 16 lanes of a row, around its end.
+template <int N>
+__device__ __forceinline__ float row_rotated(float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x120 + N, 0xf, 0xf, true));
+}
 __device__ __forceinline__ float rows_max(float x) {
   x = fmaxf(x, lane_xor16(x));
   return fmaxf(x, xhalf(x));
@@ -132,10 +137,14 @@ __device__ __forceinline__ int k_slot(int b) {
 struct RowRef {
   int page, row;
 };
+// A page number as it is followed: one outside the cache (bad_pages) as page 0.
+__device__ __forceinline__ int page_in(const PagedCache& c, int page) {
+  return (unsigned)page < (unsigned)c.num_pages ? page : 0;
+}
 __device__ __forceinline__ RowRef row_ref(const PagedCache& c, const int* table, int key, int last) {
   key = key < 0 ? 0 : key > last ? last : key;
   const int idx = page_of(c.div, key);
-  return RowRef{table[idx], key - idx * (int)c.div.size};
+  return RowRef{page_in(c, table[idx]), key - idx * (int)c.div.size};
 }
 __device__ __forceinline__ long long row_at(const PagedCache& c, RowRef r) {
   return (long long)r.page * c.page_stride + (long long)r.row * c.row_stride;
@@ -431,14 +440,15 @@ __device__ __forceinline__ void add_specials(Running<DT>& st, const float* vh, c
 
 __device__ __forceinline__ float nan_value() { return __int_as_float(0x7fc00000); }
 
-// Is a page number of slots [first, last] outside the cache?  (All threads of
-// the work group call it.)
+// Does this thread's share of the page numbers of slots [first, last] hold one
+// outside the cache?  What reads through it is NaN in the end; loads meanwhile
+// follow page_in and need not wait for the answer.
 __device__ __forceinline__ bool bad_pages(const PagedCache& c, const int* table, int first, int last) {
   bool bad = false;
   const int end = page_of(c.div, last);
   for (int i = page_of(c.div, first) + (int)threadIdx.x; i <= end; i += (int)blockDim.x)
     bad = bad || (unsigned)table[i] >= (unsigned)c.num_pages;
-  return __syncthreads_or(bad);
+  return bad;
 }
 
 // Many rows: WV waves of 16 rows each share the tiles of V.  A weight tile is the
@@ -465,7 +475,7 @@ template <class E, int DT, int WV> struct Many {
 
 // Waves per SIMD that the registers are held to: what fits without spilling.
 template <class E, int DT> constexpr int many_waves() {
-  return std::is_same<E, float>::value ? (DT <= 32 ? 4 : DT <= 64 ? 3 : 2) : DT <= 64 ? 4 : 2;
+  return std::is_same<E, float>::value ? (DT <= 64 ? 4 : 2) : DT <= 64 ? 4 : 2;
 }
 
 template <class E, int DT, int WV, bool PAGE32>
@@ -503,6 +513,7 @@ __global__ __launch_bounds__(64 * WV, (many_waves<E, DT>())) void ca_paged_atten
     if (pos_max < first && split > 0) continue;  // nothing here; the join knows
     const int end = split == io.splits - 1 || first + io.split_keys > pos_max ? pos_max + 1 : first + io.split_keys;
     const int ntiles = end > first ? (end - first + 31) / 32 : 0;
+    const bool whole_rows = io.splits == 1 || pos_max < io.split_keys;  // this split is all they see
     // (fp32: the quarter rows feed the product at the split's start, the limbs the tiles)
     const Rows<E, DT> R = load_rows<E, DT>(io, sp, h, row0 + 16 * wave + i16);
     Limbs qb[P::kF32 ? KS : 1];
@@ -529,14 +540,11 @@ __global__ __launch_bounds__(64 * WV, (many_waves<E, DT>())) void ca_paged_atten
     for (int x = 0; x < DT / 16; ++x) st.o[x] = f32x4{0.f, 0.f, 0.f, 0.f};
     if (tid < 2) special[tid] = 0;
     bool bad = false;
-    if (ntiles > 0) bad = bad_pages(c, table, first > 0 ? first - 1 : 0, end <= pos_max ? end : pos_max);
-    else __syncthreads();
-    if (bad) {
-      st.m = st.z = nan_value();
-    } else if (ntiles > 0) {
+    if (ntiles > 0) {
+      bad = bad_pages(c, table, first > 0 ? first - 1 : 0, end <= pos_max ? end : pos_max);
       // ---- where rows lie ----
       auto clamped = [&](int key) { return key < 0 ? 0 : key > pos_max ? pos_max : key; };
-      auto page_at = [&](int key) { return table[page_of(c.div, clamped(key))]; };
+      auto page_at = [&](int key) { return page_in(c, table[page_of(c.div, clamped(key))]); };
       // of a key whose page's number is known
       auto in_page = [&](int key, int page) {
         const int at = clamped(key), idx = page_of(c.div, at);
@@ -670,6 +678,7 @@ __global__ __launch_bounds__(64 * WV, (many_waves<E, DT>())) void ca_paged_atten
         float L, Rs;
         seg_shares(sl, s_carry, fast_exp2(sl), fast_exp2(s_carry), L, Rs);
         r_carry = seg ? Rs : 0.f;
+        __syncthreads();  // `special` has been cleared
         stage(0, 0);
         if (ntiles > 1) look_up(first + 32);
       }
@@ -774,11 +783,12 @@ __global__ __launch_bounds__(64 * WV, (many_waves<E, DT>())) void ca_paged_atten
       st.z = rows_sum(st.z);
       st.m = first <= R.pos ? shift - kAbove : kNegBig;
     }
+    if (__syncthreads_or(bad)) st.m = st.z = nan_value();
 
     const long long nrows = (long long)io.tokens * io.Hq;
     const float meff = st.m - weight_octaves<E>();
     if (R.row >= 0) {
-      if (io.splits == 1) {
+      if (whole_rows) {
         const float inv = st.z == 0.f ? 0.f : 1.0f / st.z;
         E* o = static_cast<E*>(io.out) + (R.row / io.Hq) * io.o_ts + (R.row % io.Hq) * io.o_hs;
 #pragma unroll
@@ -862,6 +872,7 @@ __global__ __launch_bounds__(256) void ca_paged_few_kernel(PagedAttnIO io) {
     const int first = split * io.split_keys;
     if (pos_max < first && split > 0) continue;  // the join knows
     const int end = split == io.splits - 1 || first + io.split_keys > pos_max ? pos_max + 1 : first + io.split_keys;
+    const bool whole_rows = io.splits == 1 || pos_max < io.split_keys;  // this split is all they see
     const Rows<E, DT> R = load_rows<E, DT>(io, sp, h, row0 + (i16 & (RP - 1)));
     Running<DT> st;
     st.m = kNegBig;
@@ -869,17 +880,15 @@ __global__ __launch_bounds__(256) void ca_paged_few_kernel(PagedAttnIO io) {
 #pragma unroll
     for (int x = 0; x < DT / 16; ++x) st.o[x] = f32x4{0.f, 0.f, 0.f, 0.f};
     bool bad = false;
-    if (end > first) bad = bad_pages(c, table, first > 0 ? first - 1 : 0, end <= pos_max ? end : pos_max);
-    if (bad) {
-      st.m = st.z = nan_value();
-    } else {
+    if (end > first) {
+      bad = bad_pages(c, table, first > 0 ? first - 1 : 0, end <= pos_max ? end : pos_max);
       const int step = 32 * TP;
       // Page numbers of a group: lane u < 16 tile u's, lanes 16 and 17 the
       // neighbours'.  (Only what PAGE32 needs.)
       auto group_pages = [&](int k0) {
         int key = lane < 16 ? k0 + 32 * lane : lane == 16 ? k0 - 1 : k0 + step;
         key = key < 0 ? 0 : key > pos_max ? pos_max : key;
-        return table[page_of(c.div, key)];
+        return page_in(c, table[page_of(c.div, key)]);
       };
       int ids = 0, next_ids = 0;
       auto tile_base = [&](int key, int u) {  // of a tile in one page
@@ -946,6 +955,10 @@ __global__ __launch_bounds__(256) void ca_paged_few_kernel(PagedAttnIO io) {
           for (int j = 0; j < P::kPieces; ++j)
             kn[j] = k_d + P::kVec * j < c.D ? *reinterpret_cast<const u32x4*>(p + P::kVec * j) : u32x4{0, 0, 0, 0};
         }
+        VRows<E, DT> v;
+        // where the registers have room, V's first tile is on its way early
+        constexpr bool kEarly = DT <= 64 && !P::kF32;
+        if (kEarly) load_vtile(k0, 0, v);
         f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
         auto products = [&](const KRows<E, DT>& kr, int u) {
           Rows<E, DT> Q = R;
@@ -963,8 +976,7 @@ __global__ __launch_bounds__(256) void ca_paged_few_kernel(PagedAttnIO io) {
           if (u + 2 < n) load_ktile(k0 + 32 * (u + 2), u + 2, ka);
           if (u + 1 < n) products(kb, u + 1);
         }
-        VRows<E, DT> v;
-        load_vtile(k0, 0, v);
+        if (!kEarly) load_vtile(k0, 0, v);
         f32x4 beyond = f32x4{0.f, 0.f, 0.f, 0.f};  // lane row 0: left, right
 #pragma unroll
         for (int p = 0; p < P::kPieces; ++p) {
@@ -1062,12 +1074,12 @@ __global__ __launch_bounds__(256) void ca_paged_few_kernel(PagedAttnIO io) {
         st.m = m;
       }
     }
+    if (__syncthreads_or(bad)) st.m = st.z = nan_value();
 
     const long long nrows = (long long)io.tokens * io.Hq;
     {
       // join the four waves' parts: O, then m and z
       float* join = reinterpret_cast<float*>(lds);
-      __syncthreads();
       {
         float* p = join + (wave * 16 + i16) * kJRow;
 #pragma unroll
@@ -1097,7 +1109,7 @@ __global__ __launch_bounds__(256) void ca_paged_few_kernel(PagedAttnIO io) {
           o += a * ld4(p + d);
         }
         const float meff = m - weight_octaves<E>();
-        if (io.splits == 1) {
+        if (whole_rows) {
           const float inv = z == 0.f ? 0.f : 1.0f / z;
           st4(static_cast<E*>(io.out) + (long long)(sp.t0 + t) * io.o_ts + (long long)head * io.o_hs + d, o * inv);
           if (io.stats && d == 0) {
@@ -1117,31 +1129,38 @@ __global__ __launch_bounds__(256) void ca_paged_few_kernel(PagedAttnIO io) {
   }
 }
 
-// Joins the splits of a row: DT / 4 lanes over its columns and the remaining
-// factor of 64 over the splits, WPR waves per row (four where there are many
-// splits, as for few rows: 64 splits of 16 rows took 9.6 us with one wave).
-template <class E, int DT, int WPR>
+// Joins the splits of a row: DT / 4 lanes over its columns, SUB groups of them over
+// the splits: one, those of a wave, or those of a work group (64 splits of 16
+// rows took 9.6 us with one wave per row, 4.4 with four; two splits of 65536
+// rows 23 with one, 8.5 with a group of 16 lanes).
+template <class E, int DT, int SUB>
 __global__ __launch_bounds__(256) void ca_paged_combine_kernel(PagedAttnIO io) {
-  constexpr int kQuads = DT / 4, kLanes = 64 / kQuads, kRows = 4 / WPR;
-  __shared__ float join[WPR == 1 ? 1 : 4][DT + 4];
+  constexpr int kQuads = DT / 4, kWave = 64 / kQuads;  // groups of a wave
+  constexpr int kRows = 256 / kQuads / SUB;            // rows of a work group
+  __shared__ float join[SUB > kWave ? 4 : 1][DT + 4];
   const PagedCache& c = io.c;
   const int slices = c.batch * c.heads;
   const int slice = blockIdx.x % slices, part = blockIdx.x / slices;
   const int b = slice / c.heads, h = slice - b * c.heads;
   const SeqSpan sp = seq_span(c, b, io.tokens);
-  const int rows = sp.n * io.group, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int d = lane % kQuads * 4, sub = lane / kQuads + (WPR == 1 ? 0 : wave * kLanes);
+  const int rows = sp.n * io.group;
+  const int d = threadIdx.x % kQuads * 4, lane_group = threadIdx.x / kQuads;
+  const int sub = lane_group % SUB;
   const long long nrows = (long long)io.tokens * io.Hq;
   const int parts = gridDim.x / slices;
-  // every work group of the attention kernel wrote the rows of its tile up to
-  // the last slot any of them sees: a row's splits are those up to its own slot
   for (int r0 = part * kRows; r0 < rows; r0 += kRows * parts) {
-    const int r = r0 + (WPR == 1 ? wave : 0);
-    if (WPR == 1 && r >= rows) continue;
-    const int t = r / io.group, head = h * io.group + r - t * io.group;
+    const int r = r0 + lane_group / SUB;
+    const bool ok = r < rows;
+    const int t = ok ? r / io.group : 0, head = h * io.group + (ok ? r - t * io.group : 0);
     const long long row = (long long)(sp.t0 + t) * io.Hq + head;
+    // every work group of the attention kernel wrote the rows of its tile up to
+    // the last slot any of them sees: a row's splits are those up to its own
+    // slot; a tile that one split covers wrote its results itself
+    const int tile_end = (r / io.tile_rows + 1) * io.tile_rows;
+    const int tile_last = (tile_end < rows ? tile_end : rows) - 1;
+    const bool done = !ok || sp.len - sp.n + tile_last / io.group < io.split_keys;
     const int pos = sp.len - sp.n + t;
-    int ns = pos < 0 ? 1 : pos / io.split_keys + 1;
+    int ns = done ? 0 : pos < 0 ? 1 : pos / io.split_keys + 1;
     if (ns > io.splits) ns = io.splits;
     float m = kNegBig, z = 0.f;
     f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -1153,22 +1172,25 @@ __global__ __launch_bounds__(256) void ca_paged_combine_kernel(PagedAttnIO io) {
       m = mn;
     };
 #pragma unroll 4
-    for (int s = sub; s < ns; s += kLanes * WPR) {
+    for (int s = sub; s < ns; s += SUB) {
       const long long at = s * nrows + row;
       const float2 ml = *reinterpret_cast<const float2*>(io.part_ml + 2 * at);
       add(ml.x, ml.y, d < c.D ? ld4(io.part_o + at * c.D + d) : f32x4{0.f, 0.f, 0.f, 0.f});
     }
+    if constexpr (SUB > 1) {
 #pragma unroll
-    for (int x = kQuads; x < 64; x <<= 1) {
-      const float pm = __shfl_xor(m, x), pz = __shfl_xor(z, x);
-      f32x4 po;
+      for (int x = kQuads; x < 64; x <<= 1) {
+        const float pm = __shfl_xor(m, x), pz = __shfl_xor(z, x);
+        f32x4 po;
 #pragma unroll
-      for (int y = 0; y < 4; ++y) po[y] = __shfl_xor(o[y], x);
-      add(pm, pz, po);
+        for (int y = 0; y < 4; ++y) po[y] = __shfl_xor(o[y], x);
+        add(pm, pz, po);
+      }
     }
-    if constexpr (WPR > 1) {
-      if (lane < kQuads) st4(&join[wave][d], o);
-      if (lane == 0) {
+    if constexpr (SUB > kWave) {
+      const int wave = threadIdx.x >> 6;
+      if ((threadIdx.x & 63) < kQuads) st4(&join[wave][d], o);
+      if ((threadIdx.x & 63) == 0) {
         join[wave][DT] = m;
         join[wave][DT + 1] = z;
       }
@@ -1179,12 +1201,12 @@ __global__ __launch_bounds__(256) void ca_paged_combine_kernel(PagedAttnIO io) {
 #pragma unroll
       for (int w = 0; w < 4; ++w) add(join[w][DT], join[w][DT + 1], ld4(&join[w][d]));
       __syncthreads();
-      if (wave > 0) continue;
     }
+    if (done || sub > 0) continue;
     const float inv = z == 0.f ? 0.f : 1.0f / z;
-    if (lane < kQuads && d < c.D)
+    if (d < c.D)
       st4(static_cast<E*>(io.out) + (long long)(sp.t0 + t) * io.o_ts + (long long)head * io.o_hs + d, o * inv);
-    if (io.stats && lane == 0) {
+    if (io.stats && d == 0) {
       io.stats[2 * row] = m;
       io.stats[2 * row + 1] = inv;
     }
@@ -1210,51 +1232,78 @@ __global__ __launch_bounds__(256) void ca_paged_sums_kernel(PagedAttnIO io) {
   float* sums = io.sums + (long long)b * io.sums_bs + (long long)h * io.sums_hs;
   const int len = sp.len < io.sums_len ? sp.len : io.sums_len;
   const int parts = gridDim.x / slices;
-  for (int first = part * 4 * kOwned; first < len; first += parts * 4 * kOwned) {
-    const int halo = first + 4 * kOwned < sp.len ? first + 4 * kOwned : sp.len - 1;
-    const bool bad = bad_pages(c, table, first > 0 ? first - 1 : 0, halo);
-    const int key = first + wave * kOwned - 1;  // key of slot 0
-    if (key + 1 >= len) continue;
+  for (int first = (part * 4 + wave) * kOwned; first < len; first += parts * 4 * kOwned) {
+    const int key = first - 1;  // key of slot 0
     float acc[8];
 #pragma unroll
-    for (int r = 0; r < 8; ++r) acc[r] = bad ? nan_value() : 0.f;
-    if (!bad) {
-      KRows<E, DT> kr;
-      RowRef ref[2];
+    for (int r = 0; r < 8; ++r) acc[r] = 0.f;
+    // first row that sees key + 1
+    int t0 = key + 1 - (sp.len - sp.n);
+    if (t0 < 0) t0 = 0;
+    int r0 = t0 * io.group / 16 * 16;
+    RowRef ref[2];
+    bool bad = false;
 #pragma unroll
-      for (int x = 0; x < 2; ++x) ref[x] = row_ref(c, table, key + k_slot(x), sp.len - 1);
-      load_k<E, DT>(c, kh, ref, kr);
-      // first row that sees key + 1
-      int t0 = key + 1 - (sp.len - sp.n);
-      if (t0 < 0) t0 = 0;
-      for (int r0 = t0 * io.group / 16 * 16; r0 < rows; r0 += 16) {
-        const Rows<E, DT> R = load_rows<E, DT>(io, sp, h, r0 + i16);
-        const float m = R.row >= 0 ? io.stats[2 * R.row] : 0.f;
-        const float inv = R.row >= 0 ? io.stats[2 * R.row + 1] : 0.f;
-        float s[8], w[8];
-        tile_products<E, DT>(kr, R, s);
+    for (int x = 0; x < 2; ++x) {
+      int at = key + k_slot(x);
+      at = at < 0 ? 0 : at > sp.len - 1 ? sp.len - 1 : at;
+      const int idx = page_of(c.div, at), page = table[idx];
+      bad = bad || (unsigned)page >= (unsigned)c.num_pages;
+      ref[x] = RowRef{page_in(c, page), at - idx * (int)c.div.size};
+    }
+    struct Row {
+      Rows<E, DT> q;
+      float m, inv;
+    };
+    auto load_row = [&](int r) {
+      Row o;
+      o.q = load_rows<E, DT>(io, sp, h, r + i16);
+      o.m = o.q.row >= 0 ? io.stats[2 * o.q.row] : 0.f;
+      o.inv = o.q.row >= 0 ? io.stats[2 * o.q.row + 1] : 0.f;
+      return o;
+    };
+    Row next = load_row(r0);
+    const int slot = 8 * G4 + i16;
+    const bool mine = i16 < 8 && slot > 0 && slot < 31 && key + slot < len;
+    const float before = mine ? sums[key + slot] : 0.f;
+    KRows<E, DT> kr;
+    load_k<E, DT>(c, kh, ref, kr);
+    for (; r0 < rows; r0 += 16) {
+      const Row row = next;
+      if (r0 + 16 < rows) next = load_row(r0 + 16);
+      const Rows<E, DT>& R = row.q;
+      float s[8], w[8];
+      tile_products<E, DT>(kr, R, s);
 #pragma unroll
-        for (int r = 0; r < 8; ++r) s[r] = fmaf(s[r], R.scale, -m - kShareShift);
-        const int pos_min = sp.len - sp.n + r0 / io.group, key0 = key + 8 * G4;
-        if (key < 0 || key + 31 > pos_min || r0 + 16 > rows) {
-          tile_weights<true>(s, key0, R.pos, w);
-          // a row's NaN stays out of the keys it does not see
+      for (int r = 0; r < 8; ++r) s[r] = fmaf(s[r], R.scale, -row.m - kShareShift);
+      const int pos_min = sp.len - sp.n + r0 / io.group, key0 = key + 8 * G4;
+      if (key < 0 || key + 31 > pos_min || r0 + 16 > rows) {
+        tile_weights<true>(s, key0, R.pos, w);
+        // a row's NaN stays out of the keys it does not see
 #pragma unroll
-          for (int r = 0; r < 8; ++r) acc[r] += key0 + r <= R.pos ? w[r] * inv : 0.f;
-        } else {
-          tile_weights<false>(s, key0, R.pos, w);
+        for (int r = 0; r < 8; ++r) acc[r] += key0 + r <= R.pos ? w[r] * row.inv : 0.f;
+      } else {
+        tile_weights<false>(s, key0, R.pos, w);
 #pragma unroll
-          for (int r = 0; r < 8; ++r) acc[r] += w[r] * inv;
-        }
+        for (int r = 0; r < 8; ++r) acc[r] += w[r] * row.inv;
       }
     }
+    if (wave_any(bad)) {
+#pragma unroll
+      for (int r = 0; r < 8; ++r) acc[r] = nan_value();
+    }
+    // over the 16 lanes of a row; lane r < 8 keeps slot 8 G4 + r
+    float total = 0.f;
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
-#pragma unroll
-      for (int x = 1; x < 16; x <<= 1) acc[r] += __shfl_xor(acc[r], x);
-      const int slot = 8 * G4 + r;
-      if (i16 == r && slot > 0 && slot < 31 && key + slot < len) sums[key + slot] += acc[r];
+      float x = acc[r];
+      x += row_rotated<8>(x);
+      x += row_rotated<4>(x);
+      x += row_rotated<2>(x);
+      x += row_rotated<1>(x);
+      total = i16 == r ? x : total;
     }
+    if (mine) sums[key + slot] = before + total;
   }
 }
 
@@ -1274,12 +1323,15 @@ hipError_t run_attention(const PagedAttnIO& io, hipStream_t s) {
 template <class E, int DT>
 hipError_t run_combine(const PagedAttnIO& io, hipStream_t s) {
   const long long slices = (long long)io.c.batch * io.c.heads;
-  const bool wide = io.splits > 8 * (256 / DT);  // more than two rounds of one wave
-  const long long rows = (long long)io.tokens * io.group / io.c.batch;
-  const long long per = wide ? rows : (rows + 3) / 4;
-  const dim3 grid((unsigned)(slices * (per < 1 ? 1 : per > 256 ? 256 : per))), block(256);
-  if (wide) hipLaunchKernelGGL((ca_paged_combine_kernel<E, DT, 4>), grid, block, 0, s, io);
-  else hipLaunchKernelGGL((ca_paged_combine_kernel<E, DT, 1>), grid, block, 0, s, io);
+  constexpr int kGroups = 256 / (DT / 4), kWave = kGroups / 4;
+  // a group walks at most four splits, a wave's groups eight each
+  const int sub = io.splits <= 4 ? 1 : io.splits <= 8 * kWave ? kWave : kGroups;
+  const long long rows = (long long)io.tokens * io.group / io.c.batch, each = kGroups / sub;
+  const long long per = (rows + each - 1) / each;
+  const dim3 grid((unsigned)(slices * (per < 1 ? 1 : per > 1024 ? 1024 : per))), block(256);
+  if (sub == 1) hipLaunchKernelGGL((ca_paged_combine_kernel<E, DT, 1>), grid, block, 0, s, io);
+  else if (sub == kWave) hipLaunchKernelGGL((ca_paged_combine_kernel<E, DT, kWave>), grid, block, 0, s, io);
+  else hipLaunchKernelGGL((ca_paged_combine_kernel<E, DT, kGroups>), grid, block, 0, s, io);
   return hipGetLastError();
 }
 template <class E, int DT>

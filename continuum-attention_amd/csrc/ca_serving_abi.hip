@@ -141,7 +141,7 @@ AttnPlan make_plan(int dtype, int batch, int kv_heads, int heads, int D, int tok
     // fit; a step takes about 2 us per 64 columns with the device full, and a
     // partial row 0.2 ns a column pair to write and read again.
     const bool f32 = dtype == CA_DTYPE_F32;
-    const int simd_waves = D <= 32 ? 4 : D <= 64 ? (f32 ? 3 : 4) : 2;
+    const int simd_waves = D <= 32 ? 4 : D <= 64 ? 4 : 2;
     long long per_cu = std::max(1, 4 * simd_waves / p.waves);
     if (f32) per_cu = std::min<long long>(per_cu, D <= 32 ? 4 : D <= 64 ? 2 : 1);
     const int key_tiles = std::max(1, (max_length + 31) / 32);
@@ -162,9 +162,9 @@ AttnPlan make_plan(int dtype, int batch, int kv_heads, int heads, int D, int tok
         const int cut = (key_tiles + s - 1) / s;
         double us = step_us * dealt_steps(cut, lengths, copies, per_cu * kCus);
         if (s > 1) {
-          double parts = 0;
-          for (int len : lengths) parts += (len + cut - 1) / cut;
-          us += 4 + parts / shown * slices * rows * D * 1.0e-4 / 64;
+          double parts = 0;  // row tiles that one split covers write none
+          for (int len : lengths) parts += len > cut ? (len + cut - 1) / cut : 0;
+          us += 4 + parts / shown * slices * rows * D * 2.5e-4 / 64;
         }
         if (s == 1 || us < best) {
           best = us;
@@ -279,6 +279,7 @@ int ca_paged_attention(const ca_paged_cache* cache, const void* q, long long q_t
   io.row_log = p.row_log;
   io.tile_group = p.tile_group;
   io.waves = p.waves;
+  io.tile_rows = p.tile_group ? 1 << p.row_log : 16 * p.waves;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   hipError_t err = ca::launch_paged_attention(io, cache->dtype, s);
   if (err == hipSuccess && p.splits > 1) err = ca::launch_paged_combine(io, cache->dtype, s);
