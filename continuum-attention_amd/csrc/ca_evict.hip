@@ -30,6 +30,21 @@ __device__ __forceinline__ unsigned sum_key(float x) {
   return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
 }
 
+// Sum over the 16 lanes of a row, in each of them.
+__device__ __forceinline__ int row_sum(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x128, 0xf, 0xf, true);  // rotations by 8, 4, 2, 1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x124, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x122, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x121, 0xf, 0xf, true);
+  return x;
+}
+// Sum of the 16 waves' numbers before wave `wave`.
+__device__ __forceinline__ int waves_before(const unsigned* of_wave, int wave) {
+  static_assert(kWaves == 16, "one lane row holds the waves' numbers");
+  const int l = threadIdx.x & 15;
+  return row_sum(l < wave ? (int)of_wave[l] : 0);
+}
+
 __global__ __launch_bounds__(kThreads) void ca_evict_select_kernel(EvictIO io) {
   __shared__ unsigned held[kHeld];
   __shared__ int hist[kBins];
@@ -64,13 +79,22 @@ __global__ __launch_bounds__(kThreads) void ca_evict_select_kernel(EvictIO io) {
   int need = io.budget - io.sinks - io.recent;    // of them kept
   unsigned bound = 0xffffffffu;
   if (need > 0) {
+    for (int i = tid; i < kBins; i += kThreads) hist[i] = 0;
     // the bits all sums share
     unsigned least = 0xffffffffu, most = 0;
-    for (int i = lo + tid; i < hi; i += kThreads) {
-      const unsigned k = sum_key(sums[i]);
-      if (i - lo < kHeld) held[i - lo] = k;
-      least = k < least ? k : least;
-      most = k > most ? k : most;
+    for (int i0 = lo + tid; i0 < hi; i0 += 4 * kThreads) {
+      float x[4];  // four loads on their way at a time
+#pragma unroll
+      for (int q = 0; q < 4; ++q) x[q] = i0 + q * kThreads < hi ? sums[i0 + q * kThreads] : 0.f;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int i = i0 + q * kThreads;
+        if (i >= hi) break;
+        const unsigned k = sum_key(x[q]);
+        if (i - lo < kHeld) held[i - lo] = k;
+        least = k < least ? k : least;
+        most = k > most ? k : most;
+      }
     }
 #pragma unroll
     for (int x = 32; x; x >>= 1) {
@@ -83,18 +107,18 @@ __global__ __launch_bounds__(kThreads) void ca_evict_select_kernel(EvictIO io) {
       wave_b[wave] = most;
     }
     __syncthreads();
-    least = wave_a[0];
-    most = wave_b[0];
-    for (int w = 1; w < kWaves; ++w) {
-      least = wave_a[w] < least ? wave_a[w] : least;
-      most = wave_b[w] > most ? wave_b[w] : most;
+    least = wave_a[lane & 15];
+    most = wave_b[lane & 15];
+#pragma unroll
+    for (int x = 8; x; x >>= 1) {
+      const unsigned p = __shfl_xor(least, x), q = __shfl_xor(most, x);
+      least = p < least ? p : least;
+      most = q > most ? q : most;
     }
     int bits = least == most ? 0 : 32 - __clz(least ^ most);
     unsigned value = bits == 32 ? 0u : most >> bits << bits;  // the bits fixed so far
     while (bits > 0) {
       const int width = bits < kBits ? bits : kBits, shift = bits - width;
-      for (int i = tid; i < kBins; i += kThreads) hist[i] = 0;
-      __syncthreads();
       for (int i = lo + tid; i < hi; i += kThreads) {
         const unsigned k = i - lo < kHeld ? held[i - lo] : sum_key(sums[i]);
         if (bits == 32 || (k ^ value) >> bits == 0) atomicAdd(&hist[k >> shift & ((1u << width) - 1)], 1);
@@ -103,6 +127,7 @@ __global__ __launch_bounds__(kThreads) void ca_evict_select_kernel(EvictIO io) {
       // sums above each bin, from the top: two bins a thread, the top ones first
       const int b0 = kBins - 1 - 2 * tid;
       const int c0 = hist[b0], c1 = hist[b0 - 1];
+      hist[b0] = hist[b0 - 1] = 0;  // for the next pass
       int above = c0 + c1;
 #pragma unroll
       for (int x = 1; x < 64; x <<= 1) {
@@ -111,8 +136,7 @@ __global__ __launch_bounds__(kThreads) void ca_evict_select_kernel(EvictIO io) {
       }
       if (lane == 63) wave_a[wave] = above;
       __syncthreads();
-      above -= c0 + c1;
-      for (int w = 0; w < wave; ++w) above += wave_a[w];
+      above += waves_before(wave_a, wave) - c0 - c1;
       // the one bin with fewer than `need` above it and enough with it
       if (above < need && above + c0 >= need) {
         pick[0] = b0;
@@ -125,47 +149,59 @@ __global__ __launch_bounds__(kThreads) void ca_evict_select_kernel(EvictIO io) {
       value |= (unsigned)pick[0] << shift;
       need -= pick[1];
       bits = shift;
-      __syncthreads();
     }
     bound = value;
   }
-  // in index order: those above the bound, `need` of those at it
-  int done = 0, equals = 0;
-  for (int i0 = 0; i0 < len; i0 += kThreads) {
-    const int i = i0 + tid;
-    bool above = false, equal = false;
-    if (i < len) {
-      if (i < lo || i >= hi) {
-        above = true;
-      } else if (io.budget > io.sinks + io.recent) {
-        const unsigned k = i - lo < kHeld ? held[i - lo] : sum_key(sums[i]);
-        above = k > bound;
-        equal = k == bound;
+  // In index order: those above the bound, `need` of those at it.  Each wave
+  // takes a run of slots, counts it, and writes it behind what the waves before
+  // it hold.
+  const int run = (len + 64 * kWaves - 1) / (64 * kWaves) * 64, from = wave * run;
+  const int to = from + run < len ? from + run : len;
+  auto look = [&](int i, bool& above, bool& equal) {
+    above = equal = false;
+    if (i >= to) return;
+    if (i < lo || i >= hi) {
+      above = true;
+    } else if (io.budget > io.sinks + io.recent) {
+      const unsigned k = i - lo < kHeld ? held[i - lo] : sum_key(sums[i]);
+      above = k > bound;
+      equal = k == bound;
+    }
+  };
+  int na = 0, ne = 0;
+  for (int i = from + lane; i < from + run; i += 64) {
+    bool above, equal;
+    look(i, above, equal);
+    na += __popcll(__ballot(above));
+    ne += __popcll(__ballot(equal));
+  }
+  __syncthreads();  // wave_a and wave_b have been read
+  if (lane == 0) {
+    wave_a[wave] = na;
+    wave_b[wave] = ne;
+  }
+  __syncthreads();
+  na = waves_before(wave_a, wave);
+  ne = waves_before(wave_b, wave);
+  const unsigned long long before = (1ull << lane) - 1;
+  for (int i0 = from + lane; i0 < from + run; i0 += 256) {
+    float x[4];  // four loads on their way at a time
+#pragma unroll
+    for (int q = 0; q < 4; ++q) x[q] = i0 + 64 * q < to ? sums[i0 + 64 * q] : 0.f;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int i = i0 + 64 * q;
+      bool above, equal;
+      look(i, above, equal);
+      const unsigned long long ma = __ballot(above), me = __ballot(equal);
+      const int a = na + __popcll(ma & before), e = ne + __popcll(me & before);
+      if (above || (equal && e < need)) {
+        const int at = a + (e < need ? e : need);
+        kept[at] = i;
+        new_sums[at] = x[q];
       }
-    }
-    const unsigned long long ma = __ballot(above), me = __ballot(equal);
-    if (lane == 0) {
-      wave_a[wave] = __popcll(ma);
-      wave_b[wave] = __popcll(me);
-    }
-    __syncthreads();
-    int na = done, ne = equals;
-    for (int w = 0; w < kWaves; ++w) {
-      if (w < wave) {
-        na += wave_a[w];
-        ne += wave_b[w];
-      }
-      done += wave_a[w];
-      equals += wave_b[w];
-    }
-    __syncthreads();
-    const unsigned long long before = (1ull << lane) - 1;
-    na += __popcll(ma & before);
-    ne += __popcll(me & before);
-    if (above || (equal && ne < need)) {
-      const int at = na + (ne < need ? ne : need);
-      kept[at] = i;
-      new_sums[at] = sums[i];
+      na += __popcll(ma);
+      ne += __popcll(me);
     }
   }
 }
