@@ -9,7 +9,10 @@
 // group's sum x, and
 //   y += s (sum x (16 + c) - (16 + z) sum x),
 // in fp32: the offset is about as large as the codes, so this costs two or three
-// bits of the 24.  fp32 x goes through the bf16 form in three exact bf16 limbs.
+// bits of the 24, which 16-bit results do not show.  fp32 x goes through the bf16
+// form in three exact bf16 limbs, and there c - z is formed as it is (six
+// instructions a pair instead of two), so that fp32 results keep those bits
+// (error 5.9e-7 -> 1.2e-7, a plain fp32 product's 1.1e-7).
 //
 // Tiles.  A wave takes 16 rows n and 128 columns k at a time, stored as the 1 KB that
 // it reads with one load: lane (i, r) gets the codes of row i, columns
@@ -42,6 +45,14 @@ __device__ __forceinline__ u32x4 operand(unsigned w) {
     return u32x4{(w << 6 & 0x03c003c0u) | 0x4c004c00u, (w << 2 & 0x03c003c0u) | 0x4c004c00u,
                  (w >> 2 & 0x03c003c0u) | 0x4c004c00u, (w >> 6 & 0x03c003c0u) | 0x4c004c00u};
   }
+}
+// c - z of the pairs of a word, off = 16 + z (whole numbers below 2^8: exact).
+__device__ __forceinline__ u32x4 operand_less(unsigned w, float off) {
+  u32x4 r = operand<true>(w);
+#pragma unroll
+  for (int p = 0; p < 4; ++p)
+    r[p] = cvt_pk_bf16(__uint_as_float(r[p] << 16) - off, __uint_as_float(r[p] & 0xffff0000u) - off);
+  return r;
 }
 template <bool BF>
 __device__ __forceinline__ f32x4 product(u32x4 a, u32x4 b, f32x4 c) {
@@ -93,6 +104,7 @@ __global__ __launch_bounds__(64 * kMostWaves) void ca_int4_kernel(Int4IO io) {
   constexpr bool kBf = !std::is_same<E, _Float16>::value;
   constexpr int XL = std::is_same<E, float>::value ? 3 : 1;
   constexpr int kPer = 4 / SUB;  // instructions of a group
+  constexpr bool kF32 = XL == 3;
   constexpr int kVec = 16 / sizeof(E), kPieces = 128 / kVec;  // 16-byte pieces of a row's 128 columns
   constexpr int kLoads = 16 * MT * kPieces / 64;              // of x per lane and block
   constexpr int kXRow = 128 + kVec;                           // staged row: 16 bytes of padding
@@ -130,6 +142,7 @@ __global__ __launch_bounds__(64 * kMostWaves) void ca_int4_kernel(Int4IO io) {
   struct Block {
     u32x4 codes[NT], x[kLoads];
     typename Raw4<E>::type scale[SUB][NT], zero[SUB][NT];
+    float row_zero[SUB][NT];  // fp32: of the row whose codes this lane holds
   };
   auto load = [&](int block, Block& o) {
 #pragma unroll
@@ -142,7 +155,10 @@ __global__ __launch_bounds__(64 * kMostWaves) void ca_int4_kernel(Int4IO io) {
       for (int a = 0; a < NT; ++a) {
         const long long at = (long long)g * rows + n[a] + 4 * r;
         o.scale[s][a] = ld_raw4(static_cast<const E*>(io.scales) + at);
-        if (io.zeros) o.zero[s][a] = ld_raw4(static_cast<const E*>(io.zeros) + at);
+        if constexpr (kF32)
+          o.row_zero[s][a] = io.zeros ? static_cast<const float*>(io.zeros)[(long long)g * rows + n[a] + i] : 8.f;
+        else if (io.zeros)
+          o.zero[s][a] = ld_raw4(static_cast<const E*>(io.zeros) + at);
       }
     }
     // rows past M are zero; whole aligned blocks are the rule
@@ -179,14 +195,17 @@ __global__ __launch_bounds__(64 * kMostWaves) void ca_int4_kernel(Int4IO io) {
       for (int j = kPer * s; j < kPer * s + kPer; ++j) {
         u32x4 c[NT];
 #pragma unroll
-        for (int a = 0; a < NT; ++a) c[a] = operand<kBf>(o.codes[a][j]);
+        for (int a = 0; a < NT; ++a) {
+          if constexpr (kF32) c[a] = operand_less(o.codes[a][j], 16.0f + o.row_zero[s][a]);
+          else c[a] = operand<kBf>(o.codes[a][j]);
+        }
 #pragma unroll
         for (int b = 0; b < MT; ++b) {
           u32x4 x[XL];
           operand_x<E, XL>(xs + (16 * b + i) * kXRow + 32 * j + 8 * r, x);
 #pragma unroll
           for (int l = XL - 1; l >= 0; --l) {
-            sum[b] = product<kBf>(ones, x[l], sum[b]);
+            if (!kF32) sum[b] = product<kBf>(ones, x[l], sum[b]);
 #pragma unroll
             for (int a = 0; a < NT; ++a) acc[a][b] = product<kBf>(c[a], x[l], acc[a][b]);
           }
@@ -195,11 +214,12 @@ __global__ __launch_bounds__(64 * kMostWaves) void ca_int4_kernel(Int4IO io) {
 #pragma unroll
       for (int a = 0; a < NT; ++a) {
         const f32x4 sc = raw_to_f32(o.scale[s][a], (const E*)nullptr);
-        const f32x4 off = io.zeros ? raw_to_f32(o.zero[s][a], (const E*)nullptr) + 16.0f : f32x4{24.f, 24.f, 24.f, 24.f};
+        f32x4 off = f32x4{24.f, 24.f, 24.f, 24.f};
+        if (!kF32 && io.zeros) off = raw_to_f32(o.zero[s][a], (const E*)nullptr) + 16.0f;
 #pragma unroll
         for (int b = 0; b < MT; ++b)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) y[a][b][e] = fmaf(sc[e], fmaf(-off[e], sum[b][e], acc[a][b][e]), y[a][b][e]);
+          for (int e = 0; e < 4; ++e) y[a][b][e] = fmaf(sc[e], kF32 ? acc[a][b][e] : fmaf(-off[e], sum[b][e], acc[a][b][e]), y[a][b][e]);
       }
     }
   };

@@ -31,6 +31,8 @@
 // (ca_paged_few_kernel).
 #include "ca_paged.h"
 
+#include <algorithm>
+
 namespace ca {
 
 namespace {
@@ -1320,6 +1322,12 @@ hipError_t run_attention(const PagedAttnIO& io, hipStream_t s) {
     hipLaunchKernelGGL((ca_paged_attention_kernel<E, DT, 8, PAGE32>), grid, dim3(512), 0, s, io);
   return hipGetLastError();
 }
+// Work groups of `parts` for each slice (at least one, at most 2^31 - 1 in all;
+// the kernels walk what more there is).
+unsigned grid_of(long long slices, long long parts) {
+  const long long most = ((1ll << 31) - 1) / slices;
+  return (unsigned)(slices * std::max<long long>(1, std::min(parts, most)));
+}
 template <class E, int DT>
 hipError_t run_combine(const PagedAttnIO& io, hipStream_t s) {
   const long long slices = (long long)io.c.batch * io.c.heads;
@@ -1328,7 +1336,7 @@ hipError_t run_combine(const PagedAttnIO& io, hipStream_t s) {
   const int sub = io.splits <= 4 ? 1 : io.splits <= 8 * kWave ? kWave : kGroups;
   const long long rows = (long long)io.tokens * io.group / io.c.batch, each = kGroups / sub;
   const long long per = (rows + each - 1) / each;
-  const dim3 grid((unsigned)(slices * (per < 1 ? 1 : per > 1024 ? 1024 : per))), block(256);
+  const dim3 grid(grid_of(slices, per < 1024 ? per : 1024)), block(256);
   if (sub == 1) hipLaunchKernelGGL((ca_paged_combine_kernel<E, DT, 1>), grid, block, 0, s, io);
   else if (sub == kWave) hipLaunchKernelGGL((ca_paged_combine_kernel<E, DT, kWave>), grid, block, 0, s, io);
   else hipLaunchKernelGGL((ca_paged_combine_kernel<E, DT, kGroups>), grid, block, 0, s, io);
@@ -1338,8 +1346,7 @@ template <class E, int DT>
 hipError_t run_sums(const PagedAttnIO& io, int max_length, hipStream_t s) {
   const long long slices = (long long)io.c.batch * io.c.heads;
   const long long parts = ((long long)max_length + 4 * kOwned - 1) / (4 * kOwned);
-  hipLaunchKernelGGL((ca_paged_sums_kernel<E, DT>), dim3((unsigned)(slices * (parts < 1 ? 1 : parts))),
-                     dim3(256), 0, s, io);
+  hipLaunchKernelGGL((ca_paged_sums_kernel<E, DT>), dim3(grid_of(slices, parts)), dim3(256), 0, s, io);
   return hipGetLastError();
 }
 

@@ -462,6 +462,20 @@ HeadRows head_rows(const Tensor& t) {
   return r;
 }
 
+// No two elements in one place (as far as nested strides show it).
+bool disjoint(const Tensor& t) {
+  std::vector<std::pair<int64_t, int64_t>> dims;  // stride, size
+  for (int64_t i = 0; i < t.dim(); ++i)
+    if (t.size(i) > 1) dims.emplace_back(t.stride(i), t.size(i));
+  std::sort(dims.begin(), dims.end());
+  int64_t span = 1;
+  for (const auto& d : dims) {
+    if (d.first < span) return false;
+    span = d.first * (d.second - 1) + span;
+  }
+  return true;
+}
+
 struct RotaryPlan {
   double magnitude;
   int64_t half, rotary_dim, inverse;
@@ -626,7 +640,7 @@ bool shares_memory(const Tensor& a, const Tensor& b) {
 }
 bool good_out(const Tensor& out, const Tensor& q) {
   return readable(out) && out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type() &&
-         out.device() == q.device() && out.stride(2) == 1 && !shares_memory(out, q) && !grads_needed({&out});
+         out.device() == q.device() && out.stride(2) == 1 && disjoint(out) && !shares_memory(out, q) && !grads_needed({&out});
 }
 
 py::object append(py::handle qo, py::handle ko, py::handle vo, py::handle po, py::handle to, double magnitude,
@@ -652,7 +666,8 @@ py::object append(py::handle qo, py::handle ko, py::handle vo, py::handle po, py
       (pos.scalar_type() != at::kLong && pos.scalar_type() != at::kInt) || !pos.is_contiguous())
     return py::none();
   ca_paged_cache c;
-  if (!describe(kp, vp, table, lengths, &starts, a.tokens, c) || c.heads != b.heads || c.head_dim != b.D)
+  if (!describe(kp, vp, table, lengths, &starts, a.tokens, c) || c.heads != b.heads || c.head_dim != b.D ||
+      !disjoint(kp) || c.k == c.v)
     return py::none();
   Tensor out;
   if (!oo.is_none()) {
@@ -720,7 +735,7 @@ py::object attend(py::handle qo, py::handle kpo, py::handle vpo, py::handle tabl
     sums = THPVariable_Unpack(so.ptr());
     if (!readable(sums) || sums.dim() != 3 || sums.scalar_type() != at::kFloat || sums.size(0) != c.batch ||
         sums.size(1) != c.heads || sums.numel() == 0 || sums.stride(2) != 1 || sums.device() != q.device() ||
-        sums.size(2) > (1 << 30) || grads_needed({&sums}))
+        sums.size(2) > (1 << 30) || !disjoint(sums) || grads_needed({&sums}))
       return py::none();
   }
   if (!oo.is_none()) {
@@ -755,7 +770,7 @@ py::object evict(py::handle kpo, py::handle vpo, py::handle table_o, py::handle 
   if (!plain_context() || grads_needed({&kp, &vp, &sums}) || !describe(kp, vp, table, lengths, nullptr, 0, c) ||
       !readable(sums) || sums.dim() != 3 || sums.scalar_type() != at::kFloat || sums.size(0) != c.batch ||
       sums.size(1) != c.heads || sums.numel() == 0 || sums.stride(2) != 1 || sums.device() != kp.device() ||
-      sums.size(2) > (1 << 30) || !counts(to, kp.device()) || to.dim() != 2 || to.size(0) != c.batch ||
+      sums.size(2) > (1 << 30) || !disjoint(kp) || !counts(to, kp.device()) || to.dim() != 2 || to.size(0) != c.batch ||
       budget <= 0 || budget > (1 << 30) || sinks < 0 || recent < 0 || sinks + recent > budget ||
       to.size(1) * c.page_size < budget)
     return py::none();

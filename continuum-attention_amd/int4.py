@@ -169,8 +169,14 @@ class Int4Linear(nn.Module):
         return cls(Int4Weight.quantize(linear.weight, group_size, zero_points, dtype))
 
     def forward(self, x):
+        x = x.to(self.scales.dtype)
+        if x.is_cuda and not torch.compiler.is_compiling():  # as in int4_linear
+            y = _native.torch_ext().int4(x, self.codes, self.scales, self.zeros, self.out_features,
+                                         self.in_features, self.group_size)
+            if y is not None:
+                return y
         w = Int4Weight(self.codes, self.scales, self.zeros, self.out_features, self.in_features, self.group_size)
-        return int4_linear(x.to(self.scales.dtype), w)
+        return int4_linear(x, w)
 
 
 def quantize_linears(module, group_size=128, zero_points=False, dtype=None, skip=()):

@@ -83,6 +83,16 @@ def _cache(k_pages, v_pages, page_table, lengths, starts, tokens):
     return c
 
 
+def _disjoint(t):
+    """No two elements in one place (as far as nested strides show it)."""
+    span = 1
+    for stride, size in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
+        if stride < span:
+            return False
+        span += stride * (size - 1)
+    return True
+
+
 def _gpu(name, dev):
     if dev.type != "cuda":
         raise RuntimeError(f"{name} runs on ROCm GPU and CPU tensors; got one on {dev}")
@@ -134,6 +144,8 @@ def rotary_append(q, k, v, positions, rotary, k_pages, v_pages, page_table, leng
     c = _cache(k_pages, v_pages, page_table, lengths, starts, N)
     _require(q.dtype == k_pages.dtype, f"q is {q.dtype}, the cache {k_pages.dtype}")
     _require((c.heads, c.head_dim) == tuple(k.shape[1:]), "the cache's heads and head dim differ from k's")
+    _require(_disjoint(k_pages) and k_pages.data_ptr() != v_pages.data_ptr(),
+             "k_pages and v_pages must be apart, and their rows too")
     if q.device != k_pages.device:
         raise RuntimeError("q must be on the device of the cache")
     p = _positions(positions, q.shape[:1], q.device)
@@ -169,7 +181,10 @@ def _check_out(out, q):
              "out must have q's shape and dtype")
     if out.device != q.device:
         raise RuntimeError("out must be on the device of q")
-    _require(out.stride(-1) == 1 and not out.is_neg(), "out rows must be contiguous")
+    _require(out.numel() == 0 or (out.stride(-1) == 1 and _disjoint(out)) and not out.is_neg(),
+             "out rows must be contiguous and apart")
+    if torch.is_grad_enabled() and out.requires_grad:
+        raise RuntimeError("out must not require grad")
     _require(out.numel() == 0 or out.untyped_storage().data_ptr() != q.untyped_storage().data_ptr(),
              "out must not share memory with q")
 
@@ -230,6 +245,7 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, starts, log_gain, 
                  f"weight_sums must be fp32 [{c.batch}, {c.heads}, slots]")
         _require(weight_sums.numel() == 0 or weight_sums.stride(2) == 1 or weight_sums.shape[2] == 1,
                  "weight_sums rows must be contiguous")
+        _require(_disjoint(weight_sums), "weight_sums rows must be apart")
         _require(not weight_sums.requires_grad or not torch.is_grad_enabled(), "weight_sums must not require grad")
         if weight_sums.device != dev:
             raise RuntimeError("weight_sums must be on the device of q")
@@ -313,6 +329,7 @@ def evict(k_pages, v_pages, page_table, lengths, weight_sums, new_table, budget,
              and weight_sums.shape[:2] == (c.batch, c.heads), f"weight_sums must be fp32 [{c.batch}, {c.heads}, slots]")
     if weight_sums.device != dev:
         raise RuntimeError("weight_sums must be on the device of the cache")
+    _require(_disjoint(k_pages), "the cache's rows must be apart")
     budget, sinks, recent = int(budget), int(sinks), int(recent)
     _require(budget > 0 and sinks >= 0 and recent >= 0 and sinks + recent <= budget,
              f"budget {budget} must be positive and hold {sinks} sinks and {recent} recent slots")

@@ -54,6 +54,8 @@ def test_paged_attention_refusals(ca):
     refused("weight_sums must be fp32", weight_sums=torch.zeros(2, 3, 40))
     refused("out must have", out=torch.empty(3, 4, 16, dtype=torch.bfloat16))
     refused("share memory", out=base["q"])
+    refused("apart", out=torch.empty(1, 4, 16).expand(3, 4, 16))
+    refused("apart", weight_sums=torch.zeros(1, 2, 40).expand(2, 2, 40))
     refused("no backward pass", RuntimeError, q=base["q"].clone().requires_grad_())
     refused("no backward pass", RuntimeError, gain=base["gain"].clone().requires_grad_())
     with torch.no_grad():
@@ -142,6 +144,7 @@ def test_rotary_refusals(ca):
     for args, match in (((q, k, k[:, :1], pos, rotary) + tail, "share their shape"),
                         ((q.bfloat16(), k.bfloat16(), k.bfloat16(), pos, rotary) + tail, "the cache"),
                         ((q, k[:, :1], k[:, :1], pos, rotary) + tail, "heads and head dim"),
+                        ((q, k, k, pos, rotary) + (case["k"], case["k"]) + tail[2:], "must be apart"),
                         ((q, k, k, pos, rotary) + tail[:-1] + (None,), "starts must be given")):
         with pytest.raises(ValueError, match=match):
             ca.rotary_append(*args)

@@ -171,6 +171,44 @@ def test_bad_pages_and_counts_are_not_followed(gpu_ca):
     assert torch.isfinite(out[:2].float()).all() and (out[2:] == 0).all()
 
 
+def test_shared_pages(gpu_ca):
+    """Two sequences with a common prefix in the same pages, a page named twice,
+    and their weight sums apart."""
+    case = make_cache([100, 90], [2, 3], page=32, dtype=torch.bfloat16, seed=21)
+    case["table"][1, :2] = case["table"][0, :2]
+    case["table"][0, 2] = case["table"][0, 1]
+    y, want, tol = attention64(case, with_sums=True)
+    g = on_gpu(case)
+    sums = torch.zeros(2, 2, 100, device="cuda")
+    out = attend(gpu_ca, g, weight_sums=sums)
+    assert (np.abs(out.double().cpu().numpy() - y) <= tol).all()
+    for (b, h), w in want.items():
+        # (weights add up to one per row: 2^-16 of them as in test_weight_sums)
+        assert np.abs(sums[b, h, :len(w)].double().cpu().numpy() - w).max() <= 2.0 ** -16
+
+
+def test_refusals_on_the_gpu(gpu_ca):
+    """Calls that the native entries hand back are reported as on the CPU."""
+    g = on_gpu(make_cache([40, 9], [2, 1], heads=2, group=2, D=16, page=8, dtype=torch.float32, seed=22))
+    for change, kw, error, match in (
+            ({"q": g["q"].clone().requires_grad_()}, {}, RuntimeError, "no backward pass"),
+            ({"q": g["q"].bfloat16()}, {}, ValueError, "q is"),
+            ({"table": g["table"].long()}, {}, ValueError, "32-bit"),
+            ({"lengths": g["lengths"].cpu()}, {}, RuntimeError, "device"),
+            ({"gain": g["gain"].cpu()}, {}, RuntimeError, "one device"),
+            ({}, {"out": g["q"]}, ValueError, "share memory"),
+            ({}, {"out": g["q"].clone()[:1].expand(3, 4, 16)}, ValueError, "apart"),
+            ({}, {"max_new": -2}, ValueError, "negative"),
+            ({}, {"weight_sums": torch.zeros(1, 2, 40, device="cuda").expand(2, 2, 40)}, ValueError, "apart")):
+        with pytest.raises(error, match=match):
+            attend(gpu_ca, {**g, **change}, **kw)
+    # doubles in log_gain are taken, as are parameters without grad mode
+    want = attend(gpu_ca, g)
+    assert torch.equal(attend(gpu_ca, {**g, "gain": g["gain"].double()}), want)
+    with torch.no_grad():
+        assert torch.equal(attend(gpu_ca, {**g, "gain": torch.nn.Parameter(g["gain"])}), want)
+
+
 def test_far_offsets(gpu_ca):
     """A cache of more than 2^32 bytes: pages at both its ends."""
     pages, page = 5000, 64
