@@ -828,9 +828,9 @@ __global__ __launch_bounds__(64 * WV, (many_waves<E, DT>())) void ca_paged_atten
 //
 // Tiles here own all of their 32 keys: neighbours are other columns' scores, and
 // the two beyond the group come from one more product (K rows k0 - 1 and k0 + 32 TP).
-// So tiles start at multiples of 32, and where pages do too (PAGE32) a tile lies
-// in one page: its number is read once for the wave and addresses are a scalar
-// base and a constant offset per lane.
+// So tiles start at multiples of 32, and where pages hold a multiple of 16 slots
+// (PAGE16) half a tile lies in one page: its number is read once for the wave and
+// addresses are a scalar base and a constant offset per lane.
 template <class E, int DT> struct Few {
   typedef Tile<E, DT> P;
   static constexpr int kV = 32 * P::kChunks / 64;  // 16-byte pieces of V of a lane per tile
@@ -839,7 +839,7 @@ template <class E, int DT> struct VRows {
   u32x4 v[Few<E, DT>::kV];
 };
 
-template <class E, int DT, bool PAGE32>
+template <class E, int DT, bool PAGE16>
 __global__ __launch_bounds__(256) void ca_paged_few_kernel(PagedAttnIO io) {
   typedef Tile<E, DT> P;
   constexpr int kV = Few<E, DT>::kV;
@@ -885,28 +885,35 @@ __global__ __launch_bounds__(256) void ca_paged_few_kernel(PagedAttnIO io) {
     if (end > first) {
       bad = bad_pages(c, table, first > 0 ? first - 1 : 0, end <= pos_max ? end : pos_max);
       const int step = 32 * TP;
-      // Page numbers of a group: lane u < 16 tile u's, lanes 16 and 17 the
-      // neighbours'.  (Only what PAGE32 needs.)
+      // Page numbers of a group: lane x < 32 those of its halves of tiles, lanes 32
+      // and 33 the neighbours'.  (Only what PAGE16 needs.)
       auto group_pages = [&](int k0) {
-        int key = lane < 16 ? k0 + 32 * lane : lane == 16 ? k0 - 1 : k0 + step;
+        int key = lane < 32 ? k0 + 16 * lane : lane == 32 ? k0 - 1 : k0 + step;
         key = key < 0 ? 0 : key > pos_max ? pos_max : key;
         return page_in(c, table[page_of(c.div, key)]);
       };
       int ids = 0, next_ids = 0;
-      auto tile_base = [&](int key, int u) {  // of a tile in one page
+      auto half_at = [&](int key, int x) {  // of half x of the group, its first key `key`
         const int idx = page_of(c.div, key);
-        const int page = __builtin_amdgcn_readlane(ids, u);
+        const int page = __builtin_amdgcn_readlane(ids, x);
         return (long long)page * c.page_stride + (long long)(key - idx * (int)c.div.size) * c.row_stride;
       };
+      // row x of tile u lies at from[x / 16] + x row strides; rows of a half that
+      // nothing sees stand for the first one's
+      auto halves = [&](int key, int u, long long& from0, long long& from1) {
+        from0 = half_at(key, 2 * u);
+        from1 = (key + 16 <= pos_max ? half_at(key + 16, 2 * u + 1) : from0) - 16 * c.row_stride;
+      };
       auto load_ktile = [&](int key, int u, KRows<E, DT>& out) {
-        if constexpr (PAGE32) {
-          const E* base = kh + tile_base(key, u);
+        if constexpr (PAGE16) {
+          long long from0, from1;
+          halves(key, u, from0, from1);
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            const int off = k_slot(x) * (int)c.row_stride + k_d;
+            const E* p = kh + ((k_slot(x) < 16 ? from0 : from1) + (k_slot(x) * (int)c.row_stride + k_d));
 #pragma unroll
             for (int j = 0; j < P::kPieces; ++j)
-              out.k[x][j] = k_d + P::kVec * j < c.D ? *reinterpret_cast<const u32x4*>(base + off + P::kVec * j)
+              out.k[x][j] = k_d + P::kVec * j < c.D ? *reinterpret_cast<const u32x4*>(p + P::kVec * j)
                                                     : u32x4{0, 0, 0, 0};
           }
         } else {
@@ -917,26 +924,24 @@ __global__ __launch_bounds__(256) void ca_paged_few_kernel(PagedAttnIO io) {
         }
       };
       auto load_vtile = [&](int key, int u, VRows<E, DT>& out) {
-        const E* base = vh;
-        if constexpr (PAGE32) base += tile_base(key, u);
+        long long from0 = 0, from1 = 0;
+        if constexpr (PAGE16) halves(key, u, from0, from1);
         const bool whole = key + 32 <= end;
 #pragma unroll
         for (int x = 0; x < kV; ++x) {
           const int at = lane + 64 * x, row = at / P::kChunks, d = at % P::kChunks * P::kVec;
           const bool mine = d < c.D && (whole || key + row < end);  // behind the last key: zeros
-          if constexpr (PAGE32) {
-            out.v[x] = mine ? *reinterpret_cast<const u32x4*>(base + (row * (int)c.row_stride + d)) : u32x4{0, 0, 0, 0};
-          } else {
-            const RowRef ref = row_ref(c, table, key + row, pos_max);
-            out.v[x] = mine ? *reinterpret_cast<const u32x4*>(base + row_at(c, ref) + d) : u32x4{0, 0, 0, 0};
-          }
+          const E* p;
+          if constexpr (PAGE16) p = vh + ((row < 16 ? from0 : from1) + (row * (int)c.row_stride + d));
+          else p = vh + row_at(c, row_ref(c, table, key + row, pos_max)) + d;
+          out.v[x] = mine ? *reinterpret_cast<const u32x4*>(p) : u32x4{0, 0, 0, 0};
         }
       };
       int k0 = first + wave * step;
-      if (PAGE32 && k0 < end) ids = group_pages(k0);
+      if (PAGE16 && k0 < end) ids = group_pages(k0);
       for (; k0 < end; k0 += 4 * step) {
         const int n = (end - k0 + 31) / 32 < TP ? (end - k0 + 31) / 32 : TP;  // tiles of this group
-        if (PAGE32 && k0 + 4 * step < end) next_ids = group_pages(k0 + 4 * step);
+        if (PAGE16 && k0 + 4 * step < end) next_ids = group_pages(k0 + 4 * step);
         // scores of the group, and of its two neighbours
         KRows<E, DT> ka, kb;
         u32x4 kn[P::kPieces];
@@ -945,9 +950,9 @@ __global__ __launch_bounds__(256) void ca_paged_few_kernel(PagedAttnIO io) {
           int key = i16 == 1 ? k0 + step : k0 - 1;
           key = key < 0 ? 0 : key > pos_max ? pos_max : key;
           RowRef ref;
-          if constexpr (PAGE32) {
+          if constexpr (PAGE16) {
             const int idx = page_of(c.div, key);
-            const int left = __builtin_amdgcn_readlane(ids, 16), right = __builtin_amdgcn_readlane(ids, 17);
+            const int left = __builtin_amdgcn_readlane(ids, 32), right = __builtin_amdgcn_readlane(ids, 33);
             ref = RowRef{i16 == 1 ? right : left, key - idx * (int)c.div.size};
           } else {
             ref = row_ref(c, table, key, pos_max);
@@ -1309,17 +1314,17 @@ __global__ __launch_bounds__(256) void ca_paged_sums_kernel(PagedAttnIO io) {
   }
 }
 
-template <class E, int DT, bool PAGE32>
+template <class E, int DT, bool PAGES>
 hipError_t run_attention(const PagedAttnIO& io, hipStream_t s) {
   const dim3 grid((unsigned)((long long)io.c.batch * io.c.heads * io.splits * io.row_tiles));
   if (io.tile_group)
-    hipLaunchKernelGGL((ca_paged_few_kernel<E, DT, PAGE32>), grid, dim3(256), 0, s, io);
+    hipLaunchKernelGGL((ca_paged_few_kernel<E, DT, PAGES>), grid, dim3(256), 0, s, io);
   else if (io.waves == 2)
-    hipLaunchKernelGGL((ca_paged_attention_kernel<E, DT, 2, PAGE32>), grid, dim3(128), 0, s, io);
+    hipLaunchKernelGGL((ca_paged_attention_kernel<E, DT, 2, PAGES>), grid, dim3(128), 0, s, io);
   else if (io.waves == 4)
-    hipLaunchKernelGGL((ca_paged_attention_kernel<E, DT, 4, PAGE32>), grid, dim3(256), 0, s, io);
+    hipLaunchKernelGGL((ca_paged_attention_kernel<E, DT, 4, PAGES>), grid, dim3(256), 0, s, io);
   else
-    hipLaunchKernelGGL((ca_paged_attention_kernel<E, DT, 8, PAGE32>), grid, dim3(512), 0, s, io);
+    hipLaunchKernelGGL((ca_paged_attention_kernel<E, DT, 8, PAGES>), grid, dim3(512), 0, s, io);
   return hipGetLastError();
 }
 // Work groups of `parts` for each slice (at least one, at most 2^31 - 1 in all;
@@ -1368,9 +1373,12 @@ hipError_t launch_paged_attention(const PagedAttnIO& io, int dtype, hipStream_t 
   return by_type(dtype, io.c.D, [&](auto width, auto* e) {
     typedef std::remove_pointer_t<decltype(e)> E;
     constexpr int kWidth = decltype(width)::value;
-    // pages that tiles of 32 keys never cross; offsets within a tile in 32 bits
-    const bool page32 = io.c.div.size % 32 == 0 && io.c.row_stride < 1 << 25;
-    return page32 ? run_attention<E, kWidth, true>(io, s) : run_attention<E, kWidth, false>(io, s);
+    // Pages that tiles (many rows) or their halves (few) never cross; offsets
+    // within a tile in 32 bits.  Halves for many rows as well: pages of 16 the same
+    // as looked up row by row (fp32 prompts 200 against 202 us), those of 32 and
+    // more slower for it (512 tokens over 8192 112 against 125).
+    const bool whole = io.c.div.size % (io.tile_group ? 16 : 32) == 0 && io.c.row_stride < 1 << 25;
+    return whole ? run_attention<E, kWidth, true>(io, s) : run_attention<E, kWidth, false>(io, s);
   });
 }
 hipError_t launch_paged_combine(const PagedAttnIO& io, int dtype, hipStream_t s) {
