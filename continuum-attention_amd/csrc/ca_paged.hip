@@ -27,7 +27,7 @@
 // instruction: the limb products of the training kernels cost as much time
 // once each wave has to split what it reads.
 //
-// Few rows (up to 16 per key head: single tokens) have a kernel of their own
+// Few rows (up to 8 per key head, fp32 16: single tokens) have a kernel of their own
 // (ca_paged_few_kernel).
 #include "ca_paged.h"
 
@@ -815,7 +815,7 @@ __global__ __launch_bounds__(64 * WV, (many_waves<E, DT>())) void ca_paged_atten
   }
 }
 
-// Few rows: up to 16 per key head.  One token of one head would leave 15 of a
+// Few rows: up to 8 per key head (fp32: 16).  One token of one head would leave 15 of a
 // tile's 16 columns empty, and the segment math is the longest part of a tile, so
 // the columns hold RP = 2^row_log rows times TP tiles of 32 keys: column c is row
 // c % RP over tile c / RP of a group of TP tiles.  The group's scores come from TP
@@ -1319,8 +1319,10 @@ hipError_t run_attention(const PagedAttnIO& io, hipStream_t s) {
   const dim3 grid((unsigned)((long long)io.c.batch * io.c.heads * io.splits * io.row_tiles));
   if (io.tile_group)
     hipLaunchKernelGGL((ca_paged_few_kernel<E, DT, PAGES>), grid, dim3(256), 0, s, io);
-  else if (io.waves == 2)
-    hipLaunchKernelGGL((ca_paged_attention_kernel<E, DT, 2, PAGES>), grid, dim3(128), 0, s, io);
+  else if (io.waves == 2) {
+    if constexpr (std::is_same<E, float>::value) return hipErrorInvalidValue;  // (not planned)
+    else hipLaunchKernelGGL((ca_paged_attention_kernel<E, DT, 2, PAGES>), grid, dim3(128), 0, s, io);
+  }
   else if (io.waves == 4)
     hipLaunchKernelGGL((ca_paged_attention_kernel<E, DT, 4, PAGES>), grid, dim3(256), 0, s, io);
   else

@@ -75,7 +75,13 @@ ca::PagedCache kernel_cache(const ca_paged_cache& c) {
 struct AttnPlan {
   int row_tiles, splits, split_keys, row_log, tile_group, waves;
 };
-constexpr int kFewRows = 16;  // rows per key head that share a wave's columns
+// Rows per key head that share a wave's columns.  From nine 16-bit rows on two
+// waves of 16 that share V are faster, though one of them is empty (us at 16
+// rows, shared columns / two waves: [4,4096,16,64] 34.3 / 31.6, [16,2048,16,64]
+// 47.5 / 43.4, [8,4096,8,128] 44.6 / 39.7); fp32, whose limbs take eight times
+// the shared memory, stays (47 / 58, 76 / 107, 117 / 157) and takes four waves
+// at least (20 rows of [8,4096,8,128] 157 with two, 131 with four).
+constexpr int kFewRows = 16;
 constexpr int kCus = 256;
 constexpr int kMostSplits = 128;
 
@@ -116,7 +122,8 @@ AttnPlan make_plan(int dtype, int batch, int kv_heads, int heads, int D, int tok
   long long tiles = 1;  // of rows
   int unit;             // keys that a split is a multiple of
   long long splits;
-  if (rows <= kFewRows) {
+  const bool f32 = dtype == CA_DTYPE_F32;
+  if (rows <= (f32 ? kFewRows : kFewRows / 2)) {
     p.row_log = p.waves = 0;
     while ((1 << p.row_log) < rows) ++p.row_log;
     // tiles of keys that share a wave: as many as leave the device two waves on
@@ -133,14 +140,13 @@ AttnPlan make_plan(int dtype, int batch, int kv_heads, int heads, int D, int tok
     splits = std::min<long long>(8 * kCus / slices, units / 4);
   } else {
     p.row_log = p.tile_group = 0;
-    p.waves = rows <= 32 ? 2 : rows <= 64 ? 4 : 8;
+    p.waves = rows <= 32 && !f32 ? 2 : rows <= 64 ? 4 : 8;
     const int tile_rows = 16 * p.waves;
     tiles = (rows + tile_rows - 1) / tile_rows;
     unit = 32;
     // By estimated time.  Work groups at once: those whose waves and shared memory
     // fit; a step takes about 2 us per 64 columns with the device full, and a
     // partial row 0.2 ns a column pair to write and read again.
-    const bool f32 = dtype == CA_DTYPE_F32;
     const int simd_waves = D <= 32 ? 4 : D <= 64 ? 4 : 2;
     long long per_cu = std::max(1, 4 * simd_waves / p.waves);
     if (f32) per_cu = std::min<long long>(per_cu, D <= 32 ? 4 : D <= 64 ? 2 : 1);
