@@ -15,7 +15,8 @@ struct EvictIO {
   float* new_sums;   // [batch][heads][budget], 0 behind the last kept
   int* new_lengths;  // [batch]
   int row_pieces, esize;  // 16-byte pieces of a row, bytes of an element
+  int parts;  // work groups per (sequence, head); set by the launch
 };
-hipError_t launch_evict(const EvictIO& io, hipStream_t s);
+hipError_t launch_evict(EvictIO io, hipStream_t s);
 
 }  // namespace ca

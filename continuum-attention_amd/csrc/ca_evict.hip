@@ -4,14 +4,18 @@
 // last `recent`, and of those between the ones with the largest weight sums, of
 // equal sums the earlier.  Kept rows go in their order into other pages.
 //
-// Selection: one work group per (sequence, key head) finds the last kept sum by
-// radix selection over the sums' bits in an order that integers compare (NaN
-// above all, -0 as 0): 11 bits a pass from the first bit in which any two sums
-// differ, so sums of similar size spread over the histogram's bins from its
-// first pass on.  A last pass in index order counts what is above the bound, and
-// what equals it up to the number that is left to keep.  The sums stay in shared
-// memory between the passes where they fit (one read of 4 bytes per slot).
-// Copying: 16 bytes a thread; bound by the kept rows read and written.
+// Selection: a work group finds the last kept sum of a (sequence, key head) by radix
+// selection over the sums' bits in an order that integers compare (NaN above all,
+// -0 as 0): 11 bits a pass from the first bit in which any two sums differ, so sums
+// of similar size spread over the histogram's bins from its first pass on.  The
+// sums stay in shared memory between the passes where they fit (one read of 4
+// bytes per slot).  Then its waves go through runs of slots in order: a wave
+// counts what is above the bound, and what equals it up to the number left to
+// keep, writes the numbers and copies the rows, 16 bytes a lane, as it finds
+// them.  With few (sequence, head)s several work groups select alike and share the
+// copying by chunks of 64 slots.  128 rows of 8192 sums, up to a quarter kept (64
+// columns of bf16): 32 us with four work groups a row, 36 with two; a copy kernel
+// of its own behind the selection took 17 + 17 us and the gap between the two.
 #include "ca_paged.h"
 #include "ca_evict.h"
 
@@ -21,7 +25,7 @@ namespace {
 
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
 constexpr int kBits = 11, kBins = 1 << kBits;
-constexpr int kHeld = 24576;  // sums held in shared memory (96 KB)
+constexpr int kHeld = 16384;  // sums held in shared memory (64 KB: two work groups fit a CU)
 
 // Integers in the order of the sums.
 __device__ __forceinline__ unsigned sum_key(float x) {
@@ -45,14 +49,53 @@ __device__ __forceinline__ int waves_before(const unsigned* of_wave, int wave) {
   return row_sum(l < wave ? (int)of_wave[l] : 0);
 }
 
-__global__ __launch_bounds__(kThreads) void ca_evict_select_kernel(EvictIO io) {
+// Rows from[0 .. count) to new slots first, first + 1, ..., by one wave.
+__device__ __forceinline__ void copy_rows(const PagedCache& c, const int* table, const int* new_table, char* k,
+                                          char* v, const EvictIO& io, const int* from, int first, int count) {
+  const int total = count * io.row_pieces;
+  for (int u0 = threadIdx.x & 63; u0 < total; u0 += 128) {
+    u32x4 kx[2], vx[2];
+    long long to[2];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int u = u0 + 64 * q;
+      to[q] = -1;
+      if (u >= total) continue;
+      const int row = u / io.row_pieces, piece = u - row * io.row_pieces;
+      const int src = from[row], dst = first + row;
+      const int si = page_of(c.div, src), di = page_of(c.div, dst);
+      const int sp = table[si], dp = new_table[di];
+      if ((unsigned)dp < (unsigned)c.num_pages)
+        to[q] = ((long long)dp * c.page_stride + (long long)(dst - di * (int)c.div.size) * c.row_stride) * io.esize +
+                16 * piece;
+      kx[q] = vx[q] = u32x4{~0u, ~0u, ~0u, ~0u};  // a page outside the cache: NaN in every type
+      if ((unsigned)sp < (unsigned)c.num_pages) {
+        const long long at =
+            ((long long)sp * c.page_stride + (long long)(src - si * (int)c.div.size) * c.row_stride) * io.esize +
+            16 * piece;
+        kx[q] = *reinterpret_cast<const u32x4*>(k + at);
+        vx[q] = *reinterpret_cast<const u32x4*>(v + at);
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      if (to[q] < 0) continue;
+      *reinterpret_cast<u32x4*>(k + to[q]) = kx[q];
+      *reinterpret_cast<u32x4*>(v + to[q]) = vx[q];
+    }
+  }
+}
+
+__global__ __launch_bounds__(kThreads) void ca_evict_kernel(EvictIO io) {
   __shared__ unsigned held[kHeld];
   __shared__ int hist[kBins];
   __shared__ unsigned wave_a[kWaves], wave_b[kWaves];
   __shared__ int pick[2];  // bin, sums above it
+  __shared__ int found[kWaves][64];
   const PagedCache& c = io.c;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int b = blockIdx.x / c.heads, h = blockIdx.x - b * c.heads;
+  const int slice = blockIdx.x / io.parts, part = blockIdx.x - slice * io.parts;
+  const int b = slice / c.heads, h = slice - b * c.heads;
   const long long room = (long long)c.pages_per_seq * c.div.size;
   int len = c.lengths[b];
   if (len > room) len = (int)room;
@@ -63,20 +106,16 @@ __global__ __launch_bounds__(kThreads) void ca_evict_select_kernel(EvictIO io) {
   int* kept = io.kept + out;
   float* new_sums = io.new_sums + out;
   const int keep = len < io.budget ? len : io.budget;
-  if (h == 0 && tid == 0) io.new_lengths[b] = keep;
-  for (int i = keep + tid; i < io.budget; i += kThreads) {
-    kept[i] = -1;
-    new_sums[i] = 0.f;
-  }
-  if (len <= io.budget) {
-    for (int i = tid; i < len; i += kThreads) {
-      kept[i] = i;
-      new_sums[i] = sums[i];
+  if (part == 0) {
+    if (h == 0 && tid == 0) io.new_lengths[b] = keep;
+    for (int i = keep + tid; i < io.budget; i += kThreads) {
+      kept[i] = -1;
+      new_sums[i] = 0.f;
     }
-    return;
   }
+  const bool all = len <= io.budget;
   const int lo = io.sinks, hi = len - io.recent;  // the slots that compete, sinks + recent <= budget < len
-  int need = io.budget - io.sinks - io.recent;    // of them kept
+  int need = all ? 0 : io.budget - io.sinks - io.recent;  // of them kept
   unsigned bound = 0xffffffffu;
   if (need > 0) {
     for (int i = tid; i < kBins; i += kThreads) hist[i] = 0;
@@ -160,7 +199,7 @@ __global__ __launch_bounds__(kThreads) void ca_evict_select_kernel(EvictIO io) {
   auto look = [&](int i, bool& above, bool& equal) {
     above = equal = false;
     if (i >= to) return;
-    if (i < lo || i >= hi) {
+    if (all || i < lo || i >= hi) {
       above = true;
     } else if (io.budget > io.sinks + io.recent) {
       const unsigned k = i - lo < kHeld ? held[i - lo] : sum_key(sums[i]);
@@ -184,6 +223,11 @@ __global__ __launch_bounds__(kThreads) void ca_evict_select_kernel(EvictIO io) {
   na = waves_before(wave_a, wave);
   ne = waves_before(wave_b, wave);
   const unsigned long long before = (1ull << lane) - 1;
+  const int* table = c.table + (long long)b * c.table_stride;
+  const int* new_table = io.new_table + (long long)b * io.new_table_stride;
+  char* k = static_cast<char*>(c.k) + (long long)h * c.head_stride * io.esize;
+  char* v = static_cast<char*>(c.v) + (long long)h * c.head_stride * io.esize;
+  int* mine = found[wave];
   for (int i0 = from + lane; i0 < from + run; i0 += 256) {
     float x[4];  // four loads on their way at a time
 #pragma unroll
@@ -194,79 +238,33 @@ __global__ __launch_bounds__(kThreads) void ca_evict_select_kernel(EvictIO io) {
       bool above, equal;
       look(i, above, equal);
       const unsigned long long ma = __ballot(above), me = __ballot(equal);
-      const int a = na + __popcll(ma & before), e = ne + __popcll(me & before);
-      if (above || (equal && e < need)) {
-        const int at = a + (e < need ? e : need);
-        kept[at] = i;
-        new_sums[at] = x[q];
-      }
+      const int first = na + (ne < need ? ne : need);  // new slot of the chunk's first
+      const bool take = above || (equal && ne + __popcll(me & before) < need);
       na += __popcll(ma);
       ne += __popcll(me);
-    }
-  }
-}
-
-// Kept rows into their new pages; u counts 16-byte pieces of a (sequence, head).
-template <int UNROLL>
-__global__ __launch_bounds__(256) void ca_evict_copy_kernel(EvictIO io) {
-  const PagedCache& c = io.c;
-  const int slices = c.batch * c.heads;
-  const int slice = blockIdx.x % slices, part = blockIdx.x / slices, parts = gridDim.x / slices;
-  const int b = slice / c.heads, h = slice - b * c.heads;
-  const int rows = io.new_lengths[b];
-  const int pieces = io.row_pieces;
-  const long long total = (long long)rows * pieces;
-  const int* kept = io.kept + (long long)slice * io.budget;
-  const int* table = c.table + (long long)b * c.table_stride;
-  const int* to = io.new_table + (long long)b * io.new_table_stride;
-  const char* k = static_cast<const char*>(c.k) + (long long)h * c.head_stride * io.esize;
-  const char* v = static_cast<const char*>(c.v) + (long long)h * c.head_stride * io.esize;
-  for (long long u0 = (long long)part * 256 * UNROLL; u0 < total; u0 += (long long)parts * 256 * UNROLL) {
-    u32x4 kx[UNROLL], vx[UNROLL];
-    long long dst[UNROLL];
-#pragma unroll
-    for (int x = 0; x < UNROLL; ++x) {
-      const long long u = u0 + x * 256 + threadIdx.x;
-      dst[x] = -1;
-      if (u >= total) continue;
-      const int row = (int)(u / pieces), piece = (int)(u - (long long)row * pieces);
-      const int src = kept[row];
-      const int si = page_of(c.div, src), di = page_of(c.div, row);
-      const int sp = table[si], dp = to[di];
-      if ((unsigned)dp >= (unsigned)c.num_pages) continue;
-      dst[x] = ((long long)dp * c.page_stride + (long long)(row - di * (int)c.div.size) * c.row_stride) * io.esize +
-               16 * piece;
-      kx[x] = vx[x] = u32x4{~0u, ~0u, ~0u, ~0u};  // a page outside the cache: NaN in every type
-      if ((unsigned)sp < (unsigned)c.num_pages) {
-        const long long at =
-            ((long long)sp * c.page_stride + (long long)(src - si * (int)c.div.size) * c.row_stride) * io.esize +
-            16 * piece;
-        kx[x] = *reinterpret_cast<const u32x4*>(k + at);
-        vx[x] = *reinterpret_cast<const u32x4*>(v + at);
+      if ((i - lane) / 64 % io.parts != part) continue;  // (the same for the wave)
+      const unsigned long long taken = __ballot(take);
+      const int count = __popcll(taken);
+      if (take) {
+        const int at = __popcll(taken & before);
+        kept[first + at] = i;
+        new_sums[first + at] = x[q];
+        mine[at] = i;
       }
-    }
-#pragma unroll
-    for (int x = 0; x < UNROLL; ++x) {
-      if (dst[x] < 0) continue;
-      *reinterpret_cast<u32x4*>(const_cast<char*>(k) + dst[x]) = kx[x];
-      *reinterpret_cast<u32x4*>(const_cast<char*>(v) + dst[x]) = vx[x];
+      wave_lds_sync();
+      copy_rows(c, table, new_table, k, v, io, mine, first, count);
+      wave_lds_sync();
     }
   }
 }
 
 }  // namespace
 
-hipError_t launch_evict(const EvictIO& io, hipStream_t s) {
+hipError_t launch_evict(EvictIO io, hipStream_t s) {
   const int slices = io.c.batch * io.c.heads;
-  hipLaunchKernelGGL(ca_evict_select_kernel, dim3((unsigned)slices), dim3(kThreads), 0, s, io);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
-  constexpr int kUnroll = 4;
-  const long long per = 256 * kUnroll;
-  long long parts = ((long long)io.budget * io.row_pieces + per - 1) / per;
-  const long long most = 16384 / slices > 1 ? 16384 / slices : 1;
-  parts = parts < 1 ? 1 : parts > most ? most : parts;
-  hipLaunchKernelGGL((ca_evict_copy_kernel<kUnroll>), dim3((unsigned)(slices * parts)), dim3(256), 0, s, io);
+  // two work groups fit each of 256 CUs
+  io.parts = slices >= 512 ? 1 : slices > 64 ? 512 / slices : 8;
+  hipLaunchKernelGGL(ca_evict_kernel, dim3((unsigned)(slices * io.parts)), dim3(kThreads), 0, s, io);
   return hipGetLastError();
 }
 
