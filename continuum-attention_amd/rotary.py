@@ -123,6 +123,9 @@ def _argument(q, k, q_out, k_out, positions, rotary, inverse):
     r = _native.Rotary()
     if rotary.turns.device != q.device:
         raise RuntimeError("the rotary embedding is on another device (Rotary.to)")
+    for t in (k, positions):  # saved-tensor hooks may have moved the positions
+        if t is not None and t.device != q.device:
+            raise RuntimeError("rotary_embedding: all tensors must be on the same GPU")
     r.q, r.q_out = q.data_ptr(), q_out.data_ptr()
     r.q_token_stride, r.q_head_stride, _ = q.stride()
     r.q_out_token_stride, r.q_out_head_stride, _ = q_out.stride()

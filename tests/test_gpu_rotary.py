@@ -235,3 +235,61 @@ def test_append_captured(gpu_ca):
         ke, ve = torch.zeros_like(kp), torch.zeros_like(vp)
         assert torch.equal(out, gpu_ca.rotary_append(q, k, v, pos, rotary, ke, ve, table, lens, starts))
         assert torch.equal(kp, ke) and torch.equal(vp, ve)
+
+
+def test_saved_positions_moved_away(gpu_ca):
+    """A saved-tensor hook that leaves the positions on the host: the backward
+    reports it, from the native function and the Python one."""
+    rotary = gpu_ca.Rotary(16, device="cuda")
+    pos = torch.arange(5, device="cuda")
+    for q in (torch.randn(5, 2, 16, device="cuda", requires_grad=True),
+              torch.randn(5, 2, 16, 2, device="cuda")[..., 0].requires_grad_()):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t):
+            y, _ = gpu_ca.rotary_embedding(q, None, pos, rotary)
+        with pytest.raises(RuntimeError, match="same GPU"):
+            y.sum().backward()
+        with torch.autograd.graph.save_on_cpu():
+            y, _ = gpu_ca.rotary_embedding(q, None, pos, rotary)
+        y.sum().backward()
+        close(q.grad, rotate64(torch.ones_like(q), pos, rotary, inverse=True))
+
+
+def test_positions_changed_before_the_backward(gpu_ca):
+    rotary = gpu_ca.Rotary(16, device="cuda")
+    pos = torch.arange(5, device="cuda")
+    q = torch.randn(5, 2, 16, device="cuda", requires_grad=True)
+    y, _ = gpu_ca.rotary_embedding(q, None, pos, rotary)
+    pos.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+def test_training_pass_captured(gpu_ca):
+    """Forward and backward in one graph, replayed with other values."""
+    rotary = gpu_ca.Rotary(32, layout="half", device="cuda")
+    q, k = (torch.randn(20, h, 32, device="cuda").bfloat16().requires_grad_() for h in (4, 2))
+    pos = torch.arange(20, device="cuda")
+    gq, gk = torch.randn_like(q), torch.randn_like(k)
+
+    def step():
+        yq, yk = gpu_ca.rotary_embedding(q, k, pos, rotary)
+        return [yq.detach(), yk.detach(), *torch.autograd.grad([yq, yk], [q, k], [gq, gk])]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(3):
+        with torch.no_grad():
+            q.mul_(-1.5)
+            k.add_(1.0)
+        pos.add_(1000)
+        gq.neg_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, step()))
