@@ -7,28 +7,21 @@
 // math in ca_common.h).  The rows of one key head are its new tokens times the
 // query heads that share it, r = t * group + g.
 //
-// Tiles.  A wave holds 16 rows and walks tiles of 32 key slots, of which it
-// owns the middle 30: slots 0 and 31 are the neighbours whose segments reach
-// into the tile.  So a tile depends on no other one but for the running
-// maximum, and keys can be cut anywhere (between waves, work groups, the pages
-// of the cache); 6.7% of the work is done twice for it.  The alternative, tiles
-// that carry a score and a share from the one before as the forward kernels do,
-// would need a product of its own at every cut.
+// Products on 16x16 matrix instructions, 16 rows by 32 keys at a time.  S^T = K Q^T:
+// the keys' rows are dealt so that lane row G = lane / 16 holds slots 8G .. 8G + 7
+// of query lane % 16; 16-bit K comes straight from memory into operand registers
+// (a row's D values are dealt to the four lane rows in quarters, the queries'
+// alike, so that a lane reads consecutive bytes).  O^T += V^T W^T takes the lane's
+// own weights as the other operand; V passes through shared memory, where it is
+// read transposed.  16-bit operands are exact in the 16-bit instructions; the
+// weights go as two 16-bit limbs (relative error 2^-17 in bf16, 2^-20 in fp16,
+// against half a step of 2^-9 and 2^-12 that the output's rounding makes).
 //
-// Products on 16x16 matrix instructions.  S^T = K Q^T: the keys' rows are dealt
-// so that lane row G = lane / 16 holds slots 8G .. 8G + 7 of query lane % 16; K
-// comes straight from memory into operand registers (a row's D values are dealt
-// to the four lane rows in quarters, the queries' alike, so that a lane reads
-// consecutive bytes).  O^T += V^T W^T takes the lane's own weights as the other
-// operand; V passes through shared memory, where it is read transposed.  16-bit
-// operands are exact in the 16-bit instructions; the weights go as two 16-bit
-// limbs (relative error 2^-17 in bf16, 2^-20 in fp16, against half a step of
-// 2^-9 and 2^-12 that the output's rounding makes).  fp32 operands take the fp32
-// instruction: the limb products of the training kernels cost as much time
-// once each wave has to split what it reads.
-//
-// Few rows (up to 8 per key head, fp32 16: single tokens) have a kernel of their own
-// (ca_paged_few_kernel).
+// Three kernels walk the keys: many rows (ca_paged_attention_kernel, bound by the
+// segments' vector instructions), few rows (ca_paged_few_kernel: up to 8 per key
+// head, fp32 16, single tokens above all; bound by the bytes of K and V), and the
+// weight sums (ca_paged_sums_kernel).  Keys are cut between work groups where the
+// rows alone do not fill the device, and joined by ca_paged_combine_kernel.
 #include "ca_paged.h"
 
 #include <algorithm>
@@ -37,7 +30,7 @@ namespace ca {
 
 namespace {
 
-constexpr int kOwned = 30;  // keys a tile owns
+constexpr int kOwned = 30;  // keys that a tile of the weight sums owns
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
@@ -194,7 +187,9 @@ __device__ __forceinline__ void tile_products(const KRows<E, DT>& kr, const Rows
   for (int r = 0; r < 8; ++r) s[r] = acc[r >> 2][r & 3];
 }
 
-// Weights of the lane's eight slots from their scores relative to the row's
+// Weights of the lane's eight slots of a tile that owns the 30 in its middle (slots
+// 0 and 31 are the neighbours whose segments reach into it, so that no tile
+// depends on another; 6.7% is done twice) from their scores relative to the row's
 // shift (log2 units, the factor 4 of the segment math taken off as there, so
 // that weights are in units of 2^shift).  key0: key of the lane's first slot.
 // MASK: some slot of the tile is before key 0 or behind a row's own key.
@@ -463,7 +458,10 @@ __device__ __forceinline__ bool bad_pages(const PagedCache& c, const int* table,
 //
 // fp32 goes through three bf16 limbs here: K and V are split once for all of the
 // waves when they are staged, and six bf16 products take 40% of the time of one
-// on the fp32 instruction.
+// on the fp32 instruction (two prompts of 2048 tokens 310 -> 202 us).  (Few rows
+// keep the fp32 instruction: there each wave would split what it reads.)  Not
+// kept: 16 waves a work group (197 against 196 us) and K's limbs in the order the
+// instruction reads them (half the bank conflicts, no time).
 template <class E, int DT, int WV> struct Many {
   typedef Tile<E, DT> P;
   static constexpr int kThreads = 64 * WV, kRows = 16 * WV;
@@ -475,13 +473,14 @@ template <class E, int DT, int WV> struct Many {
   static constexpr int kBytes = 2 * (P::kF32 ? 6 * kPlane * 2 : 32 * P::kRow * 2);
 };
 
-// Waves per SIMD that the registers are held to: what fits without spilling.
-template <class E, int DT> constexpr int many_waves() {
-  return std::is_same<E, float>::value ? (DT <= 64 ? 4 : 2) : DT <= 64 ? 4 : 2;
-}
+// Waves per SIMD that the registers are held to.  Four at up to 64 columns, though
+// that spills a few (16-bit 4 to 24, fp32 27 at most): with three, one work group of
+// eight waves is left per CU (512 tokens over 8192 in bf16 116 -> 175 us, two fp32
+// prompts of 2048 tokens 208 -> 232).
+template <int DT> constexpr int many_waves() { return DT <= 64 ? 4 : 2; }
 
 template <class E, int DT, int WV, bool PAGE32>
-__global__ __launch_bounds__(64 * WV, (many_waves<E, DT>())) void ca_paged_attention_kernel(PagedAttnIO io) {
+__global__ __launch_bounds__(64 * WV, (many_waves<DT>())) void ca_paged_attention_kernel(PagedAttnIO io) {
   typedef Tile<E, DT> P;
   typedef Many<E, DT, WV> M;
   constexpr int KS = DT / 32;  // 32-wide products of the scores in limbs
@@ -819,8 +818,9 @@ __global__ __launch_bounds__(64 * WV, (many_waves<E, DT>())) void ca_paged_atten
 // tile's 16 columns empty, and the segment math is the longest part of a tile, so
 // the columns hold RP = 2^row_log rows times TP tiles of 32 keys: column c is row
 // c % RP over tile c / RP of a group of TP tiles.  The group's scores come from TP
-// products into one accumulator, each with the queries zeroed outside its tile's
-// columns; the segments are then formed once for all of the group; and O^T
+// products, of each of which the columns of its tile are kept (added up with the
+// other columns' queries zeroed, a key that is not finite, behind the last one say,
+// would make other keys' scores NaN); the segments are then formed once for all of the group; and O^T
 // takes TP products again, each with the weights of its own columns.  Every
 // column keeps its own running maximum, and columns and waves are joined at the
 // end.  Per tile this leaves some 60 vector instructions of 520 with one tile at
@@ -968,14 +968,12 @@ __global__ __launch_bounds__(256) void ca_paged_few_kernel(PagedAttnIO io) {
         if (kEarly) load_vtile(k0, 0, v);
         f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
         auto products = [&](const KRows<E, DT>& kr, int u) {
-          Rows<E, DT> Q = R;
-          if (TP > 1) {
+          f32x4 part[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+          add_products<E, DT>(kr, R, part);
 #pragma unroll
-            for (int p = 0; p < P::kPieces; ++p)
+          for (int x = 0; x < 2; ++x)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) Q.q[p][e] = u_col == u ? Q.q[p][e] : 0u;
-          }
-          add_products<E, DT>(kr, Q, acc);
+            for (int e = 0; e < 4; ++e) acc[x][e] = u_col == u ? part[x][e] : acc[x][e];
         };
         for (int u = 0; u < n; u += 2) {
           if (u + 1 < n) load_ktile(k0 + 32 * (u + 1), u + 1, kb);

@@ -40,6 +40,8 @@ int check_cache(const char* op, const ca_paged_cache* c, bool starts = true) {
   if (c->table_stride < c->pages_per_seq)
     return set_error(CA_ERR_INVALID, "%s: table stride %lld below %d pages per sequence", op,
                      c->table_stride, c->pages_per_seq);
+  if (c->page_stride < 0 || c->head_stride < 0 || c->row_stride < 0)
+    return set_error(CA_ERR_INVALID, "%s: negative strides", op);
   if (!c->k || !c->v || !c->table || !c->lengths || (starts && !c->starts))
     return set_error(CA_ERR_INVALID, "%s: null pointer", op);
   if (!aligned(c->table, 4) || !aligned(c->lengths, 4) || !aligned(c->starts, 4))
@@ -91,7 +93,9 @@ size_t partial_bytes(int splits, int tokens, int heads, int D) {
 
 // Many rows: the time, in steps of one tile of one work group, that `slots` work
 // groups at once take for row tiles of given lengths (in tiles, longest first, each
-// `slices` times) cut at `cut`: each item goes to the slot that is free first.
+// `slices` times) cut at `cut`: each item goes to the slot that is free first.  (A
+// length is below 2^13 and there are at most 16 items for a slot: a few
+// megabytes at the very most.)
 int dealt_steps(int cut, const std::vector<int>& lengths, long long slices, long long slots) {
   std::vector<long long> free_at(64, 0);  // slots that become free at each step
   free_at[0] = slots;
@@ -151,22 +155,24 @@ AttnPlan make_plan(int dtype, int batch, int kv_heads, int heads, int D, int tok
     long long per_cu = std::max(1, 4 * simd_waves / p.waves);
     if (f32) per_cu = std::min<long long>(per_cu, D <= 32 ? 4 : D <= 64 ? 2 : 1);
     const int key_tiles = std::max(1, (max_length + 31) / 32);
+    const int coarse = 1 + key_tiles / 4096;  // key tiles counted as one below
     std::vector<int> lengths;  // of up to 64 row tiles (more are much alike)
     const int shown = (int)std::min<long long>(tiles, 64);
     for (int t = 0; t < shown; ++t) {
       const long long last = std::min<long long>(rows, (tiles - t * tiles / shown) * tile_rows) - 1;
       const long long keys = std::max<long long>(1, max_length - (rows - 1 - last) / group);
-      lengths.push_back((int)((keys + 31) / 32));
+      lengths.push_back((int)((keys + 32ll * coarse - 1) / (32 * coarse)));
     }
     const long long copies = slices * tiles / shown;  // work groups per length
     const double step_us = 0.55 * p.waves * per_cu / (simd_waves * 4) * 4 * std::max(1.0, D / 64.0) * (f32 ? 1.7 : 1.0);
     double best = 0;
     splits = 1;
-    if (copies > 0)
+    // (with 16 work groups for each slot the last ones cost little, cut or not)
+    if (slices * tiles < 16 * per_cu * kCus)
       for (int s : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 24, 32, 48, 64}) {
         if (s > 1 && key_tiles / s < 4) break;
-        const int cut = (key_tiles + s - 1) / s;
-        double us = step_us * dealt_steps(cut, lengths, copies, per_cu * kCus);
+        const int cut = (key_tiles + s * coarse - 1) / (s * coarse);
+        double us = step_us * coarse * dealt_steps(cut, lengths, copies, per_cu * kCus);
         if (s > 1) {
           double parts = 0;  // row tiles that one split covers write none
           for (int len : lengths) parts += len > cut ? (len + cut - 1) / cut : 0;

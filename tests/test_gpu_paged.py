@@ -129,6 +129,45 @@ def test_nothing_leaks_from_behind(gpu_ca, dtype, new):
                     assert torch.equal(got[new - 1, :, 1:], want[new - 1, :, 1:])
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("page", [16, 48, 7])
+@pytest.mark.parametrize("new,group", [(1, 1), (1, 2), (3, 1), (2, 4), (1, 16)])
+def test_tiles_that_share_a_wave(gpu_ca, dtype, page, new, group):
+    """A table wide enough that several tiles of keys share a wave's columns: the
+    results, and keys behind the last slot that are not finite, which must not
+    reach other tiles' columns."""
+    print(f"[case] page {page} new {new} group {group} {dtype}", flush=True)
+    case = make_cache([301, 70, 559], [new, 1, new], group=group, page=page, dtype=dtype, seed=page + new)
+    wide = torch.zeros(3, -(-200000 // page), dtype=torch.int32)
+    wide[:, :case["table"].shape[1]] = case["table"]
+    want = check(gpu_ca, {**case, "table": wide})
+    g = on_gpu({**case, "table": wide})
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        for b, length in enumerate((301, 70, 559)):
+            if length % page == 0:
+                continue  # no slots behind the last one
+            g["k"][case["table"][b, length // page].long(), :, length % page:] = bad
+            g["v"][case["table"][b, length // page].long(), :, length % page:] = bad
+        assert torch.equal(attend(gpu_ca, g), want)
+    if new > 1:  # the last key of a sequence: only its own row may change
+        page_id, slot = case["table"][0, 300 // page].long(), 300 % page
+        for bad in (float("nan"), float("inf"), -float("inf")):
+            for name in ("k", "v"):
+                h = {**g, name: g[name].clone()}
+                h[name][page_id, :, slot] = bad
+                got = attend(gpu_ca, h)
+                assert torch.equal(got[:new - 1], want[:new - 1]) and torch.equal(got[new:], want[new:])
+
+
+def test_many_slots_for_each_sequence(gpu_ca):
+    """The plan for a table whose pages may hold 2^30 slots, many rows each."""
+    case = make_cache([100, 50], [40, 33], group=4, page=16, seed=3)
+    for width in (1 << 16, 1 << 20):
+        wide = torch.zeros(2, width, dtype=torch.int32)
+        wide[:, :case["table"].shape[1]] = case["table"]
+        check(gpu_ca, {**case, "table": wide})
+
+
 @pytest.mark.parametrize("lengths,new", [([3, 40], [5, 2]), ([0, 40], [4, 1]), ([0, 0], [1, 1])])
 def test_rows_that_see_nothing_are_zero(gpu_ca, lengths, new):
     """More new tokens than cached slots: the first see nothing."""
