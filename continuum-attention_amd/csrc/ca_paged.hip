@@ -1327,10 +1327,10 @@ hipError_t run_attention(const PagedAttnIO& io, hipStream_t s) {
     hipLaunchKernelGGL((ca_paged_attention_kernel<E, DT, 8, PAGES>), grid, dim3(512), 0, s, io);
   return hipGetLastError();
 }
-// Work groups of `parts` for each slice (at least one, at most 2^31 - 1 in all;
-// the kernels walk what more there is).
+// Work groups of `parts` for each slice (at least one, at most 2^24 - 1 of 256
+// threads in all; the kernels walk what more there is).
 unsigned grid_of(long long slices, long long parts) {
-  const long long most = ((1ll << 31) - 1) / slices;
+  const long long most = ((1ll << 24) - 1) / slices;
   return (unsigned)(slices * std::max<long long>(1, std::min(parts, most)));
 }
 template <class E, int DT>

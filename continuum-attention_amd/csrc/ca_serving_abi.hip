@@ -20,6 +20,7 @@ int element_bytes(int dtype) {
   return dtype == CA_DTYPE_F32 ? 4 : dtype == CA_DTYPE_BF16 || dtype == CA_DTYPE_F16 ? 2 : 0;
 }
 constexpr int kMaxSlots = 1 << 30;  // slots a sequence may have: tile ends stay below 2^31
+constexpr int kMaxSlices = 1 << 21;  // (sequence, key head)s: a launch has at most 2^32 - 1 threads
 
 // A cache's numbers and pointers; `op` names the caller.
 int check_cache(const char* op, const ca_paged_cache* c, bool starts = true) {
@@ -190,8 +191,8 @@ AttnPlan make_plan(int dtype, int batch, int kv_heads, int heads, int D, int tok
   const int per = (units + (int)splits - 1) / (int)splits;
   p.splits = (units + per - 1) / per;
   p.split_keys = per * unit;
-  // at most 2^31 - 1 work groups
-  p.row_tiles = (int)std::max<long long>(1, std::min<long long>(tiles, ((1ll << 31) - 1) / (slices * p.splits)));
+  // at most 2^32 - 1 threads, 512 in a work group; each walks the row tiles behind its first
+  p.row_tiles = (int)std::max<long long>(1, std::min<long long>(tiles, ((1ll << 23) - 1) / (slices * p.splits)));
   return p;
 }
 
@@ -220,7 +221,7 @@ extern "C" {
 size_t ca_paged_attention_workspace_bytes(int dtype, int batch, int kv_heads, int heads, int head_dim, int tokens,
                                           int max_new, int max_length, int with_sums) {
   if (batch <= 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || head_dim <= 0 || tokens <= 0 || max_new < 0 ||
-      max_length < 0 || max_length > kMaxSlots || (long long)batch * kv_heads > 1 << 24)
+      max_length < 0 || max_length > kMaxSlots || (long long)batch * kv_heads > kMaxSlices)
     return 0;
   const AttnPlan p = attn_plan(dtype, batch, kv_heads, heads, head_dim, tokens, max_new, max_length);
   return partial_bytes(p.splits, tokens, heads, head_dim) + (with_sums ? stats_bytes(tokens, heads) : 0);
@@ -247,8 +248,8 @@ int ca_paged_attention(const ca_paged_cache* cache, const void* q, long long q_t
     return set_error(CA_ERR_INVALID, "%s: log_gain and sums must be 4-byte aligned", op);
   if ((long long)cache->tokens * heads * cache->head_dim > (1ll << 31) - 1)
     return set_error(CA_ERR_UNSUPPORTED, "%s: %d tokens of %d heads exceed 2^31 elements", op, cache->tokens, heads);
-  if ((long long)cache->batch * cache->heads > (1 << 24))
-    return set_error(CA_ERR_UNSUPPORTED, "%s: %d sequences of %d heads exceed 2^24", op, cache->batch, cache->heads);
+  if ((long long)cache->batch * cache->heads > kMaxSlices)
+    return set_error(CA_ERR_UNSUPPORTED, "%s: %d sequences of %d heads exceed 2^21", op, cache->batch, cache->heads);
   if (max_new < 0 || max_length < 0 || sums_len < 0)
     return set_error(CA_ERR_INVALID, "%s: negative max_new, max_length or sums_len", op);
   max_length = std::min(max_length, cache->pages_per_seq * cache->page_size);
@@ -317,8 +318,8 @@ int ca_evict(const ca_paged_cache* cache, const float* sums, long long sums_batc
   if (new_table_stride <= 0 || new_table_stride < (budget + (long long)cache->page_size - 1) / cache->page_size)
     return set_error(CA_ERR_INVALID, "%s: %lld new pages of %d slots do not hold %d", op, new_table_stride,
                      cache->page_size, budget);
-  if ((long long)cache->batch * cache->heads > (1 << 24))
-    return set_error(CA_ERR_UNSUPPORTED, "%s: %d sequences of %d heads exceed 2^24", op, cache->batch, cache->heads);
+  if ((long long)cache->batch * cache->heads > kMaxSlices)
+    return set_error(CA_ERR_UNSUPPORTED, "%s: %d sequences of %d heads exceed 2^21", op, cache->batch, cache->heads);
   ca::EvictIO io;
   io.c = kernel_cache(*cache);
   io.sums = sums;
@@ -433,7 +434,7 @@ int ca_int4_linear(const void* x, long long x_stride, const unsigned* codes, con
   if (M < 0 || N <= 0 || K <= 0) return set_error(CA_ERR_INVALID, "%s: invalid shape M=%d N=%d K=%d", op, M, N, K);
   if (group != 32 && group != 64 && (group <= 0 || group % 128))
     return set_error(CA_ERR_UNSUPPORTED, "%s: groups of %d columns (32, 64 or a multiple of 128)", op, group);
-  if ((long long)N * ((K + 127) / 128 * 128ll) > (1ll << 38) || M > (1 << 19) || K > (1 << 30) || N > (1 << 30))
+  if ((long long)N * ((K + 127) / 128 * 128ll) > (1ll << 38) || M > (1 << 19) || K > (1 << 30) || N > (1 << 26))
     return set_error(CA_ERR_UNSUPPORTED, "%s: M=%d N=%d K=%d too large", op, M, N, K);
   if (x_stride < K || y_stride < N) return set_error(CA_ERR_INVALID, "%s: row strides below the rows' lengths", op);
   if (M == 0) return CA_OK;

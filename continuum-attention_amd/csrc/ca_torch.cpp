@@ -811,7 +811,7 @@ py::object int4_product(py::handle xo, py::handle co, py::handle so, py::handle 
     rs = std::max(x.stride(0), K);
   else if (!x.is_contiguous())
     return py::none();
-  if (M > (1 << 19) || N > (1 << 30) || K > (1 << 30)) return py::none();
+  if (M > (1 << 19) || N > (1 << 26) || K > (1 << 30)) return py::none();
   Tensor y;
   {
     py::gil_scoped_release release;

@@ -125,7 +125,8 @@ def rotary_append(q, k, v, positions, rotary, k_pages, v_pages, page_table, leng
     q ``[tokens, heads, D]``, k and v ``[tokens, kv_heads, D]`` of the cache's
     dtype, positions ``[tokens]`` integers (they need not be the slots, and after
     an eviction are not).  One launch.  Two new tokens must not share a slot.
-    Slots without a page of the cache are not written.  ``out`` receives q;
+    Slots without a page of the cache are not written.  ``out`` (no other
+    argument's memory) receives q;
     without it rows that belong to no sequence are undefined.  ``max_new`` is
     accepted for symmetry with paged_attention and not needed."""
     # the plain case runs in native code (csrc/ca_torch.cpp); what it does not take is checked here
@@ -213,8 +214,11 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, starts, log_gain, 
     tokens, over the query heads of its key head, which evict ranks by.
 
     A token that sees no slot gets zeros; one that reads a page number outside
-    the cache gets NaN.  ``out`` receives the result; without it rows that belong
-    to no sequence are undefined."""
+    the cache gets NaN.  Of keys and values that are not finite, those a token does
+    not see change nothing in its row; from those it sees the row may get
+    NaN where the formula has an infinity.  ``out`` (no other argument's memory)
+    receives the result; without it rows that belong to no sequence are
+    undefined."""
     if _on_gpu(q):  # as in rotary_append
         y = _native.torch_ext().attend(q, k_pages, v_pages, page_table, lengths, starts, log_gain,
                                        -1 if max_new is None else int(max_new),
@@ -308,7 +312,8 @@ def evict(k_pages, v_pages, page_table, lengths, weight_sums, new_table, budget,
     """Cuts every sequence's cache to ``budget`` slots: of each key head the first
     ``sinks``, the last ``recent`` and, of those between, the slots with the
     largest ``weight_sums`` (``[B, kv_heads, slots]`` fp32; of equal ones the first;
-    NaN counts as the largest).  Shorter sequences are kept whole.
+    NaN counts as the largest).  Shorter sequences are kept whole; slots that
+    ``weight_sums`` does not reach are not kept.
 
     The kept rows are copied, in their order, to slots 0, 1, ... of the pages that
     ``new_table [B, new pages per sequence]`` names in the same cache; these must be
@@ -334,6 +339,7 @@ def evict(k_pages, v_pages, page_table, lengths, weight_sums, new_table, budget,
     _require(budget > 0 and sinks >= 0 and recent >= 0 and sinks + recent <= budget,
              f"budget {budget} must be positive and hold {sinks} sinks and {recent} recent slots")
     _int32("new_table", new_table, (c.batch, None), dev)
+    _require(c.batch == 1 or new_table.stride(0) >= new_table.shape[1], "new_table rows must not overlap")
     _require(new_table.shape[1] * c.page_size >= budget,
              f"{new_table.shape[1]} new pages of {c.page_size} slots do not hold {budget}")
     s = weight_sums.detach().resolve_neg()

@@ -325,3 +325,41 @@ def test_paged_cache_bookkeeping(ca):
     assert tight.counts == [12] and len(tight.owned[0]) == 3 and not tight.free
     with pytest.raises(ValueError, match="without weight_sums"):
         ca.PagedCache(1, 1, 1, 8, 12, device="cpu").evict(4)
+
+
+def test_tables_and_strides_that_would_be_read_past_their_ends(ca):
+    case = make_cache([9, 3], [1, 1], D=8, page=4, dtype=torch.float32, spare=4)
+    sums = torch.ones(2, 2, 9)
+    with pytest.raises(ValueError, match="new_table rows must not overlap"):
+        ca.evict(case["k"], case["v"], case["table"], case["lengths"], sums, case["spare"][:2].view(1, 2).expand(2, -1), 5)
+    one = case["table"][:1].expand(2, -1)
+    with pytest.raises(ValueError, match="page_table rows must not overlap"):
+        ca.evict(case["k"], case["v"], one, case["lengths"], sums, case["spare"].view(2, 2), 5)
+    with pytest.raises(ValueError, match="page_table rows must not overlap"):
+        attend(ca, {**case, "table": one})
+    lib = ca.native.load()
+    c = ca.native.PagedCache()
+    for n in ("k", "v", "table", "lengths", "starts"):
+        setattr(c, n, 4096)
+    c.dtype, c.heads, c.head_dim, c.page_size, c.num_pages, c.pages_per_seq, c.batch, c.tokens = 1, 4, 64, 16, 9, 8, 2, 3
+    for n in ("page_stride", "head_stride", "row_stride"):
+        c.page_stride, c.head_stride, c.row_stride, c.table_stride = 4096, 1024, 64, 8
+        setattr(c, n, -64)
+        assert lib.ca_paged_attention(ctypes.byref(c), 4096, 256, 64, 4, 4096, 4096, 256, 64, None, 0, 0, 0, 1, 128,
+                                      None, 0, None) == 1
+        assert b"negative strides" in lib.ca_last_error()
+    c.row_stride, c.batch = 64, 1 << 20  # 2^22 (sequence, head)s
+    assert lib.ca_paged_attention(ctypes.byref(c), 4096, 256, 64, 4, 4096, 4096, 256, 64, None, 0, 0, 0, 1, 128,
+                                  None, 0, None) == 2
+    assert lib.ca_evict(ctypes.byref(c), 4096, 0, 0, 128, 16, 0, 0, 4096, 1, 4096, 4096, 4096, None) == 2
+
+
+def test_plans_of_any_size(ca):
+    """Workspace sizes, which follow the plan of the grid, up to the limits."""
+    lib = ca.native.load()
+    for dtype in (0, 1, 2):
+        for batch, tokens, new in ((1, 1, 1), (1, 1 << 20, 1 << 20), (1 << 18, 1 << 18, 1), (4096, 1 << 20, 64),
+                                   (1, 1 << 20, 64), (3, 1 << 30, 1 << 30)):
+            for length in (0, 1, 33, 1 << 17, 1 << 24, 1 << 30):
+                n = lib.ca_paged_attention_workspace_bytes(dtype, batch, 8, 8, 64, tokens, new, length, 0)
+                assert 0 <= n <= max(1 << 30, lib.ca_workspace_cap())
