@@ -22,12 +22,17 @@
 // [16,8192] x [8192,8192] 26 us.)  x passes through shared memory for the same
 // reason: read as 256 bytes of a row by 16 lanes, handed over as operands.  Each
 // group's sums are scaled where they end.  The waves of a work group deal out the
-// columns and add up at the end in a fixed order.
+// columns and add up at the end in a fixed order.  A wave loads a block, multiplies
+// it, loads the next: other waves hide its loads.  (Two blocks a wave in flight
+// and half as many waves: [16,8192] x [8192,8192], groups of 64, 14.0 us against
+// 12.0, which is 2.9 TB/s of codes; codes alone loaded ahead: 12.9.)
 //
 // Codes of a word (eight columns): column 2 p in bits 4 p, column 2 p + 1 in bits
 // 16 + 4 p, so that a shift by 4 p lines up a pair in the two halves.  Rows of
 // codes, and of scales and zero points ([group][row]), are padded to 16.
 #include "ca_int4.h"
+
+#include <algorithm>
 
 namespace ca {
 
@@ -95,12 +100,10 @@ __device__ __forceinline__ void operand_x(const E* p, u32x4 (&out)[XL]) {
   }
 }
 
-constexpr int kMostWaves = 8;
-
 // NT: 16-row tiles of a work group, MT: 16-column (rows of x) tiles, SUB: groups
-// in 128 columns (4, 2, 1).
-template <class E, int NT, int MT, int SUB>
-__global__ __launch_bounds__(64 * kMostWaves) void ca_int4_kernel(Int4IO io) {
+// in 128 columns (4, 2, 1), WAVES: the most of a work group.
+template <class E, int NT, int MT, int SUB, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void ca_int4_kernel(Int4IO io) {
   constexpr bool kBf = !std::is_same<E, _Float16>::value;
   constexpr int XL = std::is_same<E, float>::value ? 3 : 1;
   constexpr int kPer = 4 / SUB;  // instructions of a group
@@ -109,7 +112,7 @@ __global__ __launch_bounds__(64 * kMostWaves) void ca_int4_kernel(Int4IO io) {
   constexpr int kLoads = 16 * MT * kPieces / 64;              // of x per lane and block
   constexpr int kXRow = 128 + kVec;                           // staged row: 16 bytes of padding
   constexpr int kXBytes = 16 * MT * kXRow * (int)sizeof(E), kJoinBytes = NT * MT * 16 * 17 * 4;
-  __shared__ __attribute__((aligned(16))) unsigned char lds[kMostWaves][kXBytes > kJoinBytes ? kXBytes : kJoinBytes];
+  __shared__ __attribute__((aligned(16))) unsigned char lds[WAVES][kXBytes > kJoinBytes ? kXBytes : kJoinBytes];
   const int lane = threadIdx.x & 63, i = lane & 15, r = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), waves = blockDim.x >> 6;
   const int n0 = blockIdx.x * 16 * NT, m0 = blockIdx.y * 16 * MT;
@@ -138,7 +141,7 @@ __global__ __launch_bounds__(64 * kMostWaves) void ca_int4_kernel(Int4IO io) {
     const int m = m0 + (lane + 64 * q) / kPieces;
     x_row[q] = m < io.M ? static_cast<const E*>(io.x) + (long long)m * io.x_rs + lane % kPieces * kVec : nullptr;
   }
-  // What a block of 128 columns needs, loaded one block ahead.
+  // What a block of 128 columns needs.
   struct Block {
     u32x4 codes[NT], x[kLoads];
     typename Raw4<E>::type scale[SUB][NT], zero[SUB][NT];
@@ -224,17 +227,10 @@ __global__ __launch_bounds__(64 * kMostWaves) void ca_int4_kernel(Int4IO io) {
     }
   };
   auto block_of = [&](int k) { return wave + waves * k; };
-  Block p, q;
-  int k = 0;
-  if (block_of(0) < blocks) load(block_of(0), p);
-  while (block_of(k) < blocks) {
-    const bool more = block_of(k + 1) < blocks;
-    if (more) load(block_of(k + 1), q);
+  Block p;
+  for (int k = 0; block_of(k) < blocks; ++k) {
+    load(block_of(k), p);
     add(p);
-    if (!more) break;
-    if (block_of(k + 2) < blocks) load(block_of(k + 2), p);
-    add(q);
-    k += 2;
   }
   wave_lds_sync();
   float* join = reinterpret_cast<float*>(lds[wave]);
@@ -257,27 +253,39 @@ __global__ __launch_bounds__(64 * kMostWaves) void ca_int4_kernel(Int4IO io) {
 }
 
 template <class E, int NT, int MT>
-hipError_t run_sub(const Int4IO& io, dim3 grid, dim3 block, hipStream_t s) {
-  if (io.group == 32) hipLaunchKernelGGL((ca_int4_kernel<E, NT, MT, 4>), grid, block, 0, s, io);
-  else if (io.group == 64) hipLaunchKernelGGL((ca_int4_kernel<E, NT, MT, 2>), grid, block, 0, s, io);
-  else hipLaunchKernelGGL((ca_int4_kernel<E, NT, MT, 1>), grid, block, 0, s, io);
+hipError_t run_sub(const Int4IO& io, dim3 grid, hipStream_t s) {
+  const int blocks = (io.K + 127) / 128;
+  auto launch = [&](auto kernel, int most) {
+    hipLaunchKernelGGL(kernel, grid, dim3(64 * std::min(blocks, most)), 0, s, io);
+  };
+  // 16 waves where there is a work group for each CU at most, unless groups of 32
+  // take too many registers; with more work groups eight are faster (us with 16 /
+  // 8: [64,1024] x [4096,1024] bf16 6.5 / 5.0, [256,4096] x [4096,4096] 46 / 38)
+  const bool few = (long long)grid.x * grid.y <= 256;
+  if (io.group == 32) {
+    if constexpr (NT == 2) return hipErrorInvalidValue;  // (not asked for)
+    else launch(ca_int4_kernel<E, NT, MT, 4, 8>, 8);
+  } else if (io.group == 64 && few) launch(ca_int4_kernel<E, NT, MT, 2, 16>, 16);
+  else if (io.group == 64) launch(ca_int4_kernel<E, NT, MT, 2, 8>, 8);
+  else if (few) launch(ca_int4_kernel<E, NT, MT, 1, 16>, 16);
+  else launch(ca_int4_kernel<E, NT, MT, 1, 8>, 8);
   return hipGetLastError();
 }
 template <class E>
 hipError_t run_int4(const Int4IO& io, hipStream_t s) {
-  const int blocks = (io.K + 127) / 128;
-  const dim3 block(64 * (blocks < kMostWaves ? blocks : kMostWaves));
   // fp32 rows take twice the shared memory: 16 at a time
   const int mt = io.M <= 16 || sizeof(E) == 4 ? 1 : 2;
   const unsigned my = (io.M + 16 * mt - 1) / (16 * mt);
   const int tiles = (io.N + 15) / 16;
   if constexpr (sizeof(E) == 2) {
-    if (mt == 2) return run_sub<E, 1, 2>(io, dim3(tiles, my), block, s);
-    // two tiles share x where that still leaves a work group for each of 256 CUs
-    // ([16,8192] x [8192,8192] 16.4 -> 15.5 us; [1,1024] x [4096,1024] 3.6 -> 4.2)
-    if (tiles >= 512) return run_sub<E, 2, 1>(io, dim3((tiles + 1) / 2, my), block, s);
+    if (mt == 2) return run_sub<E, 1, 2>(io, dim3(tiles, my), s);
+    // two tiles share x where that still leaves a work group for each of 256 CUs, and
+    // groups of 32, which take the registers, stay with one ([16,8192] x [8192,8192],
+    // us with one / two, groups of 32: 16.7 / 17.5, of 64: 13.9 / 12.0, of 128: 13.2 /
+    // 11.1; [1,1024] x [4096,1024] 3.6 / 4.2)
+    if (tiles >= 512 && io.group > 32) return run_sub<E, 2, 1>(io, dim3((tiles + 1) / 2, my), s);
   }
-  return run_sub<E, 1, 1>(io, dim3(tiles, my), block, s);
+  return run_sub<E, 1, 1>(io, dim3(tiles, my), s);
 }
 
 }  // namespace

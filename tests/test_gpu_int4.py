@@ -128,3 +128,11 @@ def test_quantize_and_module(gpu_ca, zero_points):
     x = torch.randn(3, 200, device="cuda")
     with torch.no_grad():
         assert torch.equal(mod(x), gpu_ca.int4_linear(x, w))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("g", [32, 64, 128])
+@pytest.mark.parametrize("M,N", [(1, 5000), (9, 5000), (1, 8200), (5, 8208), (20, 100), (40, 3001), (33, 8200)])
+def test_grids_past_the_compute_units(gpu_ca, dtype, g, M, N):
+    """Work groups of either size: up to one for each compute unit, and more."""
+    check(gpu_ca, M, N, 2500, g, True, dtype)
