@@ -4,6 +4,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <new>
 #include <vector>
 
 #include "ca_evict.h"
@@ -157,33 +158,37 @@ AttnPlan make_plan(int dtype, int batch, int kv_heads, int heads, int D, int tok
     if (f32) per_cu = std::min<long long>(per_cu, D <= 32 ? 4 : D <= 64 ? 2 : 1);
     const int key_tiles = std::max(1, (max_length + 31) / 32);
     const int coarse = 1 + key_tiles / 4096;  // key tiles counted as one below
-    std::vector<int> lengths;  // of up to 64 row tiles (more are much alike)
-    const int shown = (int)std::min<long long>(tiles, 64);
-    for (int t = 0; t < shown; ++t) {
-      const long long last = std::min<long long>(rows, (tiles - t * tiles / shown) * tile_rows) - 1;
-      const long long keys = std::max<long long>(1, max_length - (rows - 1 - last) / group);
-      lengths.push_back((int)((keys + 32ll * coarse - 1) / (32 * coarse)));
-    }
-    const long long copies = slices * tiles / shown;  // work groups per length
-    const double step_us = 0.55 * p.waves * per_cu / (simd_waves * 4) * 4 * std::max(1.0, D / 64.0) * (f32 ? 1.7 : 1.0);
-    double best = 0;
     splits = 1;
-    // (with 16 work groups for each slot the last ones cost little, cut or not)
-    if (slices * tiles < 16 * per_cu * kCus)
-      for (int s : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 24, 32, 48, 64}) {
-        if (s > 1 && key_tiles / s < 4) break;
-        const int cut = (key_tiles + s * coarse - 1) / (s * coarse);
-        double us = step_us * coarse * dealt_steps(cut, lengths, copies, per_cu * kCus);
-        if (s > 1) {
-          double parts = 0;  // row tiles that one split covers write none
-          for (int len : lengths) parts += len > cut ? (len + cut - 1) / cut : 0;
-          us += 4 + parts / shown * slices * rows * D * 2.5e-4 / 64;
-        }
-        if (s == 1 || us < best) {
-          best = us;
-          splits = s;
-        }
+    try {
+      std::vector<int> lengths;  // of up to 64 row tiles (more are much alike)
+      const int shown = (int)std::min<long long>(tiles, 64);
+      for (int t = 0; t < shown; ++t) {
+        const long long last = std::min<long long>(rows, (tiles - t * tiles / shown) * tile_rows) - 1;
+        const long long keys = std::max<long long>(1, max_length - (rows - 1 - last) / group);
+        lengths.push_back((int)((keys + 32ll * coarse - 1) / (32 * coarse)));
       }
+      const long long copies = slices * tiles / shown;  // work groups per length
+      const double step_us = 0.55 * p.waves * per_cu / (simd_waves * 4) * 4 * std::max(1.0, D / 64.0) * (f32 ? 1.7 : 1.0);
+      double best = 0;
+      // (with 16 work groups for each slot the last ones cost little, cut or not)
+      if (slices * tiles < 16 * per_cu * kCus)
+        for (int s : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 24, 32, 48, 64}) {
+          if (s > 1 && key_tiles / s < 4) break;
+          const int cut = (key_tiles + s * coarse - 1) / (s * coarse);
+          double us = step_us * coarse * dealt_steps(cut, lengths, copies, per_cu * kCus);
+          if (s > 1) {
+            double parts = 0;  // row tiles that one split covers write none
+            for (int len : lengths) parts += len > cut ? (len + cut - 1) / cut : 0;
+            us += 4 + parts / shown * slices * rows * D * 2.5e-4 / 64;
+          }
+          if (s == 1 || us < best) {
+            best = us;
+            splits = s;
+          }
+        }
+    } catch (const std::bad_alloc&) {
+      splits = 1;  // no memory for the estimate
+    }
   }
   const int units = std::max(1, (max_length + unit - 1) / unit);
   splits = std::max<long long>(1, std::min<long long>({splits, kMostSplits, units}));
@@ -207,10 +212,11 @@ AttnPlan attn_plan(int dtype, int batch, int kv_heads, int heads, int D, int tok
   const long long key[9] = {dtype, batch, kv_heads, heads, D, tokens, max_new, max_length, (long long)ca_workspace_cap()};
   for (unsigned i = 0; i < std::min(used, 16u); ++i)
     if (std::equal(key, key + 9, kept[i].key)) return kept[i].plan;
+  const AttnPlan plan = make_plan(dtype, batch, kv_heads, heads, D, tokens, max_new, max_length);
   Entry& e = kept[used++ % 16];
-  e.plan = make_plan(dtype, batch, kv_heads, heads, D, tokens, max_new, max_length);
+  e.plan = plan;
   std::copy(key, key + 9, e.key);
-  return e.plan;
+  return plan;
 }
 size_t stats_bytes(int tokens, int heads) { return ((size_t)tokens * heads * 2 * sizeof(float) + 255) & ~(size_t)255; }
 
